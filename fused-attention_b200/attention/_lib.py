@@ -12,12 +12,13 @@ reference's `ct.launch(torch.cuda.current_stream(), ...)` (attention/fused/fused
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfa_sm100.so")
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 
 
@@ -49,6 +50,10 @@ SIGNATURES = {
     "fa_bwd_dq": [_VP, _VP, _VP, _VP, _FP, _FP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _VP, _VP],
     "fa_bwd_noalloc": [_VP, _VP, _VP, _VP, _VP, _FP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _VP, _VP],
     "fa_unfused_fwd": [_VP, _VP, _VP, _VP, _FP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP],
+    "fa_norm_rope_fwd": [_VP, _VP, _VP],
+    "fa_norm_rope_bwd": [_VP, _VP, _VP],
+    "fa_append_kv": [_VP, _VP, _VP],
+    "fa_paged_attention": [_VP, _VP, _VP],
 }
 _RESTYPES = {"fa_strerror": ctypes.c_char_p, "fa_last_cuda_error": ctypes.c_char_p}
 
@@ -59,8 +64,12 @@ _status = {}  # device index -> int32[4] status tensor
 DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
 
 
+BAD_INDEX = 111  # status code: an index that the kernel read lies outside its table
+
+
 class KernelError(RuntimeError):
-    """A device-side pipeline wait timed out (the kernel stopped instead of hanging)."""
+    """A device-side pipeline wait timed out (the kernel stopped instead of hanging), or an index read
+    by a kernel lies outside its table (the kernel stayed inside its buffers)."""
 
 
 def load():
@@ -109,6 +118,9 @@ def check_status(device=None, reset=True):
     if vals[0] != 0:
         if reset:
             st.zero_()
+        if vals[0] == BAD_INDEX:
+            raise KernelError(f"a position, page, sequence length or offset lies outside its table "
+                              f"(code {vals[0]}, cta {vals[1]}, index {vals[2]})")
         raise KernelError(f"device pipeline error code {vals[0]} (cta {vals[1]}, thread {vals[2]})")
 
 
@@ -206,6 +218,59 @@ def unfused_fwd(q, k, v, o, s, p):
     B, H, S, D = q.shape
     _launch(q, [("fa_unfused_fwd", (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), s.data_ptr(),
                                     p.data_ptr(), B, H, k.shape[1], S, D, _dtype_code(q)))])
+
+
+# ---- norm + rotary positions, paged cache, attention over it: arguments travel in one struct
+# (include/fa_sm100.h); a packed bytes object converts to its pointer.
+NORM_ROPE_ARGS = struct.Struct("@16P14q15if")
+APPEND_ARGS = struct.Struct("@13P6qd18i")
+PAGED_ARGS = struct.Struct("@11P5q9if")
+ROPE_WORKSPACE_ROWS = 296
+F32_CODE = 2
+
+
+def paged_workspace_bytes(head_dim):
+    return 40960 * head_dim + 131072
+
+
+def norm_rope_fwd(q, packed):
+    _launch(q, [("fa_norm_rope_fwd", (packed,))])
+
+
+def norm_rope_bwd(q, packed):
+    _launch(q, [("fa_norm_rope_bwd", (packed,))])
+
+
+def append_kv(k, packed):
+    _launch(k, [("fa_append_kv", (packed,))])
+
+
+def paged_attention(q, packed):
+    _launch(q, [("fa_paged_attention", (packed,))])
+
+
+def rows16(x):
+    """x as the kernels take 16-bit rows: contiguous in its last dimension, base and strides on 16-byte
+    boundaries (a copy where it is not), and its other strides (0 for dimensions of size 1)."""
+    size, stride = x.shape, x.stride()
+    ok = stride[-1] == 1 and x.data_ptr() % 16 == 0
+    strides = []
+    for n, s in zip(size[:-1], stride[:-1]):
+        if n == 1:
+            s = 0
+        elif s % 8 or s < 0:
+            ok = False
+        strides.append(s)
+    if ok:
+        return x, strides
+    x = x.clone(memory_format=torch.contiguous_format)
+    return x, [0 if n == 1 else s for n, s in zip(x.shape[:-1], x.stride()[:-1])]
+
+
+def aligned16(x):
+    """x contiguous with its base on a 16-byte boundary (a copy where it is not)."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 def load_by_path():

@@ -6,6 +6,8 @@
 #include <atomic>
 #include <cstdint>
 
+#include "../../include/fa_sm100.h"
+
 namespace fa {
 
 // Parameters of one forward launch (plain values; tensor maps travel separately as
@@ -56,6 +58,106 @@ struct UnfParams {
   float sm_scale;     // 1 / sqrt(D)
 };
 
+// Parameters of the per-head norm + rotary kernels (fa_rope.cu).
+constexpr int kRopeMaxAxes = 4;
+constexpr int kRopeBwdBlocks = FA_ROPE_WORKSPACE_ROWS;
+struct RopeParams {
+  const void* q;
+  const void* k;
+  const void* q_weight;      // [D], nullptr: rotation only
+  const void* k_weight;
+  const float* cos;          // [max_pos, D / 2]
+  const float* sin;
+  const void* pos;           // int32 / int64, nullptr: token n of each row of the batch is at n
+  void* q_out;               // forward: contiguous [B, H, N, D]
+  void* k_out;
+  const void* dq_out;        // backward: contiguous [B, H, N, D]
+  const void* dk_out;
+  void* dq;
+  void* dk;
+  void* dq_weight;           // [D], nullptr: not asked for
+  void* dk_weight;
+  float* workspace;          // [kRopeBwdBlocks, D]
+  long long q_stride[3];     // batch, head, token (elements)
+  long long k_stride[3];
+  long long dq_stride[3];
+  long long dk_stride[3];
+  long long pos_axis_stride;
+  long long pos_batch_stride;
+  long long tokens;          // B * N
+  int* status;
+  int H, H_kv, N;
+  int max_pos;
+  int axes;
+  int section_start[kRopeMaxAxes];  // first pair of each axis
+  int pos64, weight_f32;
+  int range_heads, q_ranges, q_blocks;  // set by the launchers
+  float eps;
+};
+
+// Parameters of the append kernel (fa_append.cu).
+struct AppendParams {
+  const void* k;             // [T, H_kv, D], strides below
+  const void* v;
+  uint8_t* k_pages;          // [num_pages, H_kv, page_size, D] e4m3
+  uint8_t* v_pages;
+  float* k_scales;           // [num_pages, H_kv]
+  float* v_scales;
+  const int* block_table;    // [B, width], rows table_stride apart
+  const int* seq_lens;       // [B], new tokens included
+  const int* offsets;        // [B + 1], nullptr: one token per sequence
+  const float* cos;          // [max_pos, D / 2], nullptr: no rotation
+  const float* sin;
+  const void* pos;           // [axes, T], nullptr: the token's place in its sequence
+  const void* k_weight;      // [D], nullptr: no norm
+  long long k_stride[2];     // token, head (elements)
+  long long v_stride[2];
+  long long table_stride;
+  long long pos_axis_stride;
+  double eps;
+  int* status;
+  int T, B, width, num_pages, H_kv, page_size;
+  int max_pos, axes;
+  int section_start[kRopeMaxAxes];
+  int pos64, weight_f32;
+  int window;                // tokens of a block, set by the launcher
+};
+
+// A cut tile of rows: its opening part is in `slot`, the others in the first slots of the blocks after.
+struct PagedJoin {
+  int parts;                 // 0: nothing to join
+  int slot;
+  int token;                 // flat index of the sequence's first token
+  int head;                  // K/V head
+  int row, rows;
+};
+
+// Parameters of attention over the paged cache (fa_paged.cu).
+constexpr int kPagedUnit = 64;
+struct PagedParams {
+  const void* q;             // [T, H, D], strides below
+  const uint8_t* k_pages;
+  const uint8_t* v_pages;
+  const float* k_scales;
+  const float* v_scales;
+  const int* block_table;
+  const int* seq_lens;
+  const int* offsets;
+  void* out;                 // [T, H, D], strides below
+  float* lse;                // [T, H] or nullptr
+  float* parts;              // workspace: [2 * blocks, rows, D]
+  float2* part_ml;           // [2 * blocks, rows]
+  PagedJoin* joins;          // [blocks]
+  long long q_stride[2];     // token, head (elements)
+  long long out_stride[2];
+  long long table_stride;
+  int* status;
+  int T, B, num_pages, H_kv, group, page_size;
+  int capacity;              // tokens that a row of the table can name
+  int bf16;
+  float scale_log2;          // log2(e) * softmax scale
+};
+
 // Work units (heads, head pairs) whose tiles are launched heavy-first together: up to 16 units,
 // about 64 MiB of K/V at S = 8192, D = 128, so the heads in flight keep their K/V in the 126 MB L2.
 #ifndef FA_WORK_BAND
@@ -94,6 +196,15 @@ inline cudaError_t opt_in_smem(Kernel kernel, int bytes, std::atomic<bool> (&don
 // FA_ERR_* code of a failed runtime query).
 int cuda_fail(cudaError_t e);
 int check_device();
+
+// Launchers of the norm + rotary kernels; D in {32, 64, 128}.
+cudaError_t launch_rope_fwd(RopeParams p, int D, bool bf16, bool interleaved, cudaStream_t stream);
+cudaError_t launch_rope_bwd(RopeParams p, int D, bool bf16, bool interleaved, cudaStream_t stream);
+
+cudaError_t launch_append(AppendParams p, int D, bool bf16, bool interleaved, cudaStream_t stream);
+int paged_row_tile(const PagedParams& p);
+int paged_blocks(const PagedParams& p);  // size of the split kernel's grid
+cudaError_t launch_paged(const PagedParams& p, int D, int blocks, cudaStream_t stream);
 
 // Launchers implemented in the kernel translation units.  They return a cudaError_t.
 cudaError_t launch_fwd(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,

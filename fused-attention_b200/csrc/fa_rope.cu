@@ -1,0 +1,462 @@
+// Per-head RMS norm of queries and keys with the rotary position rotation in the same pass,
+// forward and backward, for sm_100a.
+//
+//   r = 1 / sqrt(mean(x^2) + eps),  y = x r w            (skipped where no weight is given)
+//   pair (a, b) of y at position p:  z = (a c - b s, a s + b c),  c, s = cos/sin[p(axis of pair), pair]
+//   backward, dz given:  dy = (da c + db s, db c - da s),  g = dy w,
+//     dx = r (g - x r^2 mean(g x)),   dw = sum over rows of dy x r
+// A pair is (i, i + D/2), or (2i, 2i + 1) when interleaved.  Sums and products are float32; each
+// output is rounded once.
+//
+// Bound: memory.  Every element is read and written once (backward: x and dz read, dx written), so
+// the layout is chosen for wide accesses and for reading the tables once per token instead of once
+// per row: a group of D/16 lanes owns a token, keeps its 8 cosines and 8 sines per lane in
+// registers and walks heads of that token, 16 elements (two 16-byte accesses) a lane and row.  The
+// pairs a lane needs are all its own, so only the row sums cross lanes (log2(D/16) shuffles).
+// kUnroll rows are loaded before the first is used.  Few tokens are spread out by giving each group
+// fewer heads (the host picks heads per group).
+// The weight gradients are summed in registers over a block's rows, then over the block's groups,
+// and written as one row per block; a second kernel adds those rows in a fixed order, so results do
+// not depend on timing.
+#include "fa_internal.h"
+#include "fa_sm100.cuh"
+
+namespace fa {
+namespace {
+
+constexpr int kRopeThreads = 256;
+
+// 8 consecutive 16-bit elements -> float32.
+template <bool BF16>
+__device__ __forceinline__ void widen8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint4 narrow8(const float (&f)[8]) {
+  return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]),
+                    pack2<BF16>(f[6], f[7]));
+}
+
+// A lane's 16 elements as 8 pairs: lo = first members, hi = second members.  `v0` and `v1` are the
+// lane's two 8-element vectors: [8l, +8) and [D/2 + 8l, +8), or [16l, +8) and [16l + 8, +8).
+template <bool BF16, bool INTER>
+__device__ __forceinline__ void to_pairs(const uint4& v0, const uint4& v1, float (&lo)[8], float (&hi)[8]) {
+  if constexpr (INTER) {
+    float a[8], b[8];
+    widen8<BF16>(v0, a);
+    widen8<BF16>(v1, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = a[2 * i];
+      hi[i] = a[2 * i + 1];
+      lo[4 + i] = b[2 * i];
+      hi[4 + i] = b[2 * i + 1];
+    }
+  } else {
+    widen8<BF16>(v0, lo);
+    widen8<BF16>(v1, hi);
+  }
+}
+
+template <bool BF16, bool INTER>
+__device__ __forceinline__ void from_pairs(const float (&lo)[8], const float (&hi)[8], uint4& v0, uint4& v1) {
+  if constexpr (INTER) {
+    v0 = make_uint4(pack2<BF16>(lo[0], hi[0]), pack2<BF16>(lo[1], hi[1]), pack2<BF16>(lo[2], hi[2]),
+                    pack2<BF16>(lo[3], hi[3]));
+    v1 = make_uint4(pack2<BF16>(lo[4], hi[4]), pack2<BF16>(lo[5], hi[5]), pack2<BF16>(lo[6], hi[6]),
+                    pack2<BF16>(lo[7], hi[7]));
+  } else {
+    v0 = narrow8<BF16>(lo);
+    v1 = narrow8<BF16>(hi);
+  }
+}
+
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One tensor of the call (queries or keys).
+template <bool BWD>
+struct RopeSide {
+  const uint16_t* x;
+  const uint16_t* dz;
+  uint16_t* out;       // z forward, dx backward
+  const void* w;
+  long long xs[3];     // strides of x: batch, head, token
+  long long os[3];     // strides of out
+  int heads;
+};
+
+template <bool BWD>
+__device__ __forceinline__ RopeSide<BWD> rope_side(const RopeParams& p, bool key) {
+  RopeSide<BWD> s;
+  s.x = static_cast<const uint16_t*>(key ? p.k : p.q);
+  s.dz = static_cast<const uint16_t*>(key ? p.dk_out : p.dq_out);
+  s.out = static_cast<uint16_t*>(BWD ? (key ? p.dk : p.dq) : (key ? p.k_out : p.q_out));
+  s.w = key ? p.k_weight : p.q_weight;
+  s.heads = key ? p.H_kv : p.H;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    s.xs[i] = key ? p.k_stride[i] : p.q_stride[i];
+    s.os[i] = key ? p.dk_stride[i] : p.dq_stride[i];
+  }
+  return s;
+}
+
+// Element offsets of a lane's two vectors inside a row.
+template <int D, bool INTER>
+__device__ __forceinline__ void lane_offsets(int l, int& o0, int& o1) {
+  o0 = INTER ? 16 * l : 8 * l;
+  o1 = INTER ? 16 * l + 8 : D / 2 + 8 * l;
+}
+
+template <int D, bool BF16, bool INTER>
+__device__ __forceinline__ void load_weight(const void* w, bool f32, int l, float (&wl)[8], float (&wh)[8]) {
+  int o0, o1;
+  lane_offsets<D, INTER>(l, o0, o1);
+  if (w == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wl[i] = wh[i] = 1.f;
+  } else if (f32) {
+    const float* f = static_cast<const float*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wl[i] = INTER ? f[o0 + 2 * i] : f[o0 + i];
+      wh[i] = INTER ? f[o0 + 2 * i + 1] : f[o1 + i];
+    }
+  } else {
+    const uint16_t* h = static_cast<const uint16_t*>(w);
+    to_pairs<BF16, INTER>(*reinterpret_cast<const uint4*>(h + o0), *reinterpret_cast<const uint4*>(h + o1), wl, wh);
+  }
+}
+
+// Position of token (b, n) on one axis, kept inside the table: an index outside it records
+// kDevBadIndex and uses row 0.
+__device__ __forceinline__ int rope_position(const RopeParams& p, int axis, int b, int n) {
+  long long v;
+  if (p.pos == nullptr) {
+    v = n;
+  } else {
+    const long long at = axis * p.pos_axis_stride + b * p.pos_batch_stride + n;
+    v = p.pos64 ? static_cast<const long long*>(p.pos)[at] : static_cast<const int*>(p.pos)[at];
+  }
+  if (v < 0 || v >= p.max_pos) {
+    record_error(p.status, kDevBadIndex, n);
+    v = 0;
+  }
+  return static_cast<int>(v);
+}
+
+template <int D>
+__device__ __forceinline__ void load_angles(const RopeParams& p, int b, int n, int l, float (&c)[8], float (&s)[8]) {
+  if (p.axes == 1) {
+    const size_t at = static_cast<size_t>(rope_position(p, 0, b, n)) * (D / 2) + 8 * l;
+    const float4* pc = reinterpret_cast<const float4*>(p.cos + at);
+    const float4* ps = reinterpret_cast<const float4*>(p.sin + at);
+    const float4 c0 = pc[0], c1 = pc[1], s0 = ps[0], s1 = ps[1];
+    c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w;
+    c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
+    s[0] = s0.x; s[1] = s0.y; s[2] = s0.z; s[3] = s0.w;
+    s[4] = s1.x; s[5] = s1.y; s[6] = s1.z; s[7] = s1.w;
+  } else {
+    int row[kRopeMaxAxes];
+#pragma unroll
+    for (int a = 0; a < kRopeMaxAxes; ++a) row[a] = a < p.axes ? rope_position(p, a, b, n) : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int pair = 8 * l + i;
+      int r = row[0];
+#pragma unroll
+      for (int a = 1; a < kRopeMaxAxes; ++a)
+        if (pair >= p.section_start[a]) r = row[a];
+      const size_t at = static_cast<size_t>(r) * (D / 2) + pair;
+      c[i] = p.cos[at];
+      s[i] = p.sin[at];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------- forward
+// grid: x = token blocks, y = head ranges (first the queries', then the keys').
+template <int D, bool BF16, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads) rope_fwd_kernel(const RopeParams p) {
+  constexpr int LPR = D / 16;
+  constexpr int kGroups = kRopeThreads / LPR;
+  constexpr int kUnroll = 4;
+  const int status = ld_status(p.status);  // looked at before the first store
+  const int l = threadIdx.x % LPR;
+  const long long token = static_cast<long long>(blockIdx.x) * kGroups + threadIdx.x / LPR;
+  const bool key = static_cast<int>(blockIdx.y) >= p.q_ranges;
+  const int range = key ? blockIdx.y - p.q_ranges : blockIdx.y;
+  const RopeSide<false> s = rope_side<false>(p, key);
+  const int h0 = range * p.range_heads, h1 = min(s.heads, h0 + p.range_heads);
+  const bool live = token < p.tokens;  // whole groups; the others stay for the shuffles
+  const int b = live ? static_cast<int>(token / p.N) : 0;
+  const int n = live ? static_cast<int>(token - static_cast<long long>(b) * p.N) : 0;
+  int o0, o1;
+  lane_offsets<D, INTER>(l, o0, o1);
+  const uint16_t* x = s.x + b * s.xs[0] + n * s.xs[2];
+  uint16_t* z = s.out + (static_cast<long long>(b) * s.heads * p.N + n) * D;
+  float wl[8], wh[8], c[8], sn[8];
+  load_weight<D, BF16, INTER>(s.w, p.weight_f32, l, wl, wh);
+  load_angles<D>(p, b, n, l, c, sn);
+  const bool norm = s.w != nullptr;
+  for (int h = h0; h < h1; h += kUnroll) {
+    uint4 v0[kUnroll], v1[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (live && h + u < h1) {
+        const uint16_t* row = x + (h + u) * s.xs[1];
+        v0[u] = *reinterpret_cast<const uint4*>(row + o0);
+        v1[u] = *reinterpret_cast<const uint4*>(row + o1);
+      } else {
+        v0[u] = v1[u] = make_uint4(0, 0, 0, 0);
+      }
+    if (status != 0) return;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float lo[8], hi[8];
+      to_pairs<BF16, INTER>(v0[u], v1[u], lo, hi);
+      if (norm) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(lo[i], lo[i], fmaf(hi[i], hi[i], sum));
+        const float r = rsqrtf(group_sum<LPR>(sum) * (1.f / D) + p.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          lo[i] = lo[i] * r * wl[i];
+          hi[i] = hi[i] * r * wh[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = lo[i], e = hi[i];
+        lo[i] = a * c[i] - e * sn[i];
+        hi[i] = a * sn[i] + e * c[i];
+      }
+      if (live && h + u < h1) {
+        uint4 r0, r1;
+        from_pairs<BF16, INTER>(lo, hi, r0, r1);
+        uint16_t* row = z + static_cast<long long>(h + u) * p.N * D;
+        *reinterpret_cast<uint4*>(row + o0) = r0;
+        *reinterpret_cast<uint4*>(row + o1) = r1;
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------- backward
+// Blocks [0, q_blocks) walk the queries' units (token block, head range), the rest the keys'; each
+// leaves its sum of dw (float32 [D]) in row blockIdx.x of the workspace.
+template <int D, bool BF16, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads, 2) rope_bwd_kernel(const RopeParams p) {
+  constexpr int LPR = D / 16;
+  constexpr int kGroups = kRopeThreads / LPR;
+  constexpr int kUnroll = 2;
+  __shared__ float part[kRopeThreads / 32][D];
+  if (__syncthreads_or(ld_status(p.status)) != 0) return;
+  const bool key = static_cast<int>(blockIdx.x) >= p.q_blocks;
+  const int block = key ? blockIdx.x - p.q_blocks : blockIdx.x;
+  const int blocks = key ? gridDim.x - p.q_blocks : p.q_blocks;
+  const RopeSide<true> s = rope_side<true>(p, key);
+  const int ranges = (s.heads + p.range_heads - 1) / p.range_heads;
+  const long long token_blocks = (p.tokens + kGroups - 1) / kGroups;
+  const int l = threadIdx.x % LPR;
+  int o0, o1;
+  lane_offsets<D, INTER>(l, o0, o1);
+  const bool norm = s.w != nullptr;
+  float wl[8], wh[8], dl[8], dh[8];
+  load_weight<D, BF16, INTER>(s.w, p.weight_f32, l, wl, wh);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dl[i] = dh[i] = 0.f;
+  for (long long unit = block; unit < token_blocks * ranges; unit += blocks) {
+    const int range = static_cast<int>(unit % ranges);
+    const long long token = unit / ranges * kGroups + threadIdx.x / LPR;
+    const bool live = token < p.tokens;
+    const int b = live ? static_cast<int>(token / p.N) : 0;
+    const int n = live ? static_cast<int>(token - static_cast<long long>(b) * p.N) : 0;
+    const int h0 = range * p.range_heads, h1 = min(s.heads, h0 + p.range_heads);
+    const uint16_t* x = s.x + b * s.xs[0] + n * s.xs[2];
+    const uint16_t* dz = s.dz + (static_cast<long long>(b) * s.heads * p.N + n) * D;
+    uint16_t* dx = s.out + b * s.os[0] + n * s.os[2];
+    float c[8], sn[8];
+    load_angles<D>(p, b, n, l, c, sn);
+    for (int h = h0; h < h1; h += kUnroll) {
+      uint4 x0[kUnroll], x1[kUnroll], z0[kUnroll], z1[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (live && h + u < h1) {
+          const uint16_t* xr = x + (h + u) * s.xs[1];
+          const uint16_t* zr = dz + static_cast<long long>(h + u) * p.N * D;
+          x0[u] = *reinterpret_cast<const uint4*>(xr + o0);
+          x1[u] = *reinterpret_cast<const uint4*>(xr + o1);
+          z0[u] = *reinterpret_cast<const uint4*>(zr + o0);
+          z1[u] = *reinterpret_cast<const uint4*>(zr + o1);
+        } else {
+          x0[u] = x1[u] = z0[u] = z1[u] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        float lo[8], hi[8];
+        to_pairs<BF16, INTER>(z0[u], z1[u], lo, hi);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // dy: the rotation turned back
+          const float a = lo[i], e = hi[i];
+          lo[i] = a * c[i] + e * sn[i];
+          hi[i] = e * c[i] - a * sn[i];
+        }
+        if (norm) {
+          float xl[8], xh[8], sum = 0.f, dot = 0.f;
+          to_pairs<BF16, INTER>(x0[u], x1[u], xl, xh);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            sum = fmaf(xl[i], xl[i], fmaf(xh[i], xh[i], sum));
+            dot = fmaf(lo[i] * wl[i], xl[i], fmaf(hi[i] * wh[i], xh[i], dot));
+          }
+          const float r = rsqrtf(group_sum<LPR>(sum) * (1.f / D) + p.eps);
+          const float t = group_sum<LPR>(dot) * (1.f / D) * r * r;
+          // rows outside the tensor were loaded as zeros: they add nothing to dw
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dl[i] = fmaf(lo[i], xl[i] * r, dl[i]);
+            dh[i] = fmaf(hi[i], xh[i] * r, dh[i]);
+            lo[i] = r * (lo[i] * wl[i] - xl[i] * t);
+            hi[i] = r * (hi[i] * wh[i] - xh[i] * t);
+          }
+        }
+        if (live && h + u < h1) {
+          uint4 r0, r1;
+          from_pairs<BF16, INTER>(lo, hi, r0, r1);
+          uint16_t* row = dx + (h + u) * s.os[1];
+          *reinterpret_cast<uint4*>(row + o0) = r0;
+          *reinterpret_cast<uint4*>(row + o1) = r1;
+        }
+      }
+    }
+  }
+  if (!norm) return;  // uniform over the block
+  // dw of the block: over the warp's groups, then over the warps
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) {
+      dl[i] += __shfl_xor_sync(0xffffffffu, dl[i], o);
+      dh[i] += __shfl_xor_sync(0xffffffffu, dh[i], o);
+    }
+  const int warp = threadIdx.x / 32;
+  if (threadIdx.x % 32 < LPR) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      part[warp][INTER ? o0 + 2 * i : o0 + i] = dl[i];
+      part[warp][INTER ? o0 + 2 * i + 1 : o1 + i] = dh[i];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRopeThreads / 32; ++w) sum += part[w][threadIdx.x];
+    p.workspace[static_cast<size_t>(blockIdx.x) * D + threadIdx.x] = sum;
+  }
+}
+
+// dw[d] = sum of the blocks' rows, in a fixed order.  grid: x = D / 32 column blocks, y = queries,
+// keys; 32 threads of a column each add every 32nd row.
+__global__ void __launch_bounds__(1024) rope_dw_kernel(const RopeParams p, int D, int blocks, bool bf16) {
+  __shared__ float part[32][33];
+  if (__syncthreads_or(ld_status(p.status)) != 0) return;
+  const bool key = blockIdx.y != 0;
+  void* out = key ? p.dk_weight : p.dq_weight;
+  if (out == nullptr) return;
+  const int col = blockIdx.x * 32 + threadIdx.x % 32, at = threadIdx.x / 32;
+  const int first = key ? p.q_blocks : 0, last = key ? blocks : p.q_blocks;
+  float sum = 0.f;
+  for (int r = first + at; r < last; r += 32) sum += p.workspace[static_cast<size_t>(r) * D + col];
+  part[at][threadIdx.x % 32] = sum;
+  __syncthreads();
+  if (at == 0) {
+    sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) sum += part[r][threadIdx.x];
+    if (p.weight_f32)
+      static_cast<float*>(out)[col] = sum;
+    else if (bf16)
+      static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(sum);
+    else
+      static_cast<__half*>(out)[col] = __float2half_rn(sum);
+  }
+}
+
+constexpr int groups_per_block(int D) { return kRopeThreads / (D / 16); }
+
+}  // namespace
+
+// Heads per group: all of them while the token blocks alone fill the GPU (the tables are then read
+// once per token), else as few as it takes to make about four blocks per SM.
+static int rope_range_heads(const RopeParams& p, int D) {
+  const long long token_blocks = (p.tokens + groups_per_block(D) - 1) / groups_per_block(D);
+  int heads = p.H > p.H_kv ? p.H : p.H_kv;
+  while (heads > 1 && token_blocks * ((p.H + heads - 1) / heads + (p.H_kv + heads - 1) / heads) < 4 * 148)
+    heads = (heads + 1) / 2;
+  return heads;
+}
+
+cudaError_t launch_rope_fwd(RopeParams p, int D, bool bf16, bool interleaved, cudaStream_t stream) {
+  p.range_heads = rope_range_heads(p, D);
+  p.q_ranges = (p.H + p.range_heads - 1) / p.range_heads;
+  const int k_ranges = (p.H_kv + p.range_heads - 1) / p.range_heads;
+  const dim3 grid(static_cast<unsigned>((p.tokens + groups_per_block(D) - 1) / groups_per_block(D)), p.q_ranges + k_ranges);
+#define FA_ROPE_CASE(DD, BB, II)                                  \
+  if (D == DD && bf16 == BB && interleaved == II) {               \
+    rope_fwd_kernel<DD, BB, II><<<grid, kRopeThreads, 0, stream>>>(p); \
+    return cudaGetLastError();                                    \
+  }
+#define FA_ROPE_CASES(DD) \
+  FA_ROPE_CASE(DD, false, false) FA_ROPE_CASE(DD, false, true) FA_ROPE_CASE(DD, true, false) FA_ROPE_CASE(DD, true, true)
+  FA_ROPE_CASES(32)
+  FA_ROPE_CASES(64)
+  FA_ROPE_CASES(128)
+#undef FA_ROPE_CASE
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_rope_bwd(RopeParams p, int D, bool bf16, bool interleaved, cudaStream_t stream) {
+  p.range_heads = rope_range_heads(p, D);
+  const long long token_blocks = (p.tokens + groups_per_block(D) - 1) / groups_per_block(D);
+  const long long q_units = token_blocks * ((p.H + p.range_heads - 1) / p.range_heads);
+  const long long k_units = token_blocks * ((p.H_kv + p.range_heads - 1) / p.range_heads);
+  // one wave of blocks, shared out by the number of heads
+  const long long k_share = p.H_kv == 0 ? 0 : (kRopeBwdBlocks * static_cast<long long>(p.H_kv) + p.H + p.H_kv - 1) / (p.H + p.H_kv);
+  const long long q_share = kRopeBwdBlocks - k_share;
+  p.q_blocks = static_cast<int>(q_units < q_share ? q_units : q_share);
+  const int blocks = p.q_blocks + static_cast<int>(k_units < k_share ? k_units : k_share);
+#define FA_ROPE_CASE(DD, BB, II)                                  \
+  if (D == DD && bf16 == BB && interleaved == II)                 \
+    rope_bwd_kernel<DD, BB, II><<<blocks, kRopeThreads, 0, stream>>>(p);
+  FA_ROPE_CASES(32)
+  FA_ROPE_CASES(64)
+  FA_ROPE_CASES(128)
+#undef FA_ROPE_CASE
+#undef FA_ROPE_CASES
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || (p.dq_weight == nullptr && p.dk_weight == nullptr)) return e;
+  rope_dw_kernel<<<dim3(D / 32, 2), 1024, 0, stream>>>(p, D, blocks, bf16);
+  return cudaGetLastError();
+}
+
+}  // namespace fa

@@ -53,6 +53,7 @@ enum DeviceError : int {
   kDevTimeoutDrain = 107,   // teardown waiting for in-flight copies / MMAs
   kDevTimeoutBwd = 108,     // backward pipeline wait
   kDevSmemLayout = 109,     // dynamic shared memory start leaves too little alignment slack
+  kDevBadIndex = 111,       // a position, page, length or offset lies outside its table
   kDevTestStall = 110,      // failure-detection test build: the injected wait ran out
   kDevAborted = 199,        // another CTA already failed; this one stopped early
 };

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define FA_ABI_VERSION 1
+#define FA_ABI_VERSION 2
 
 #if defined(__GNUC__)
 #define FA_API __attribute__((visibility("default")))
@@ -50,7 +50,7 @@ enum fa_status_code {
 /* Capacity of fa_bwd_noalloc's static scratch: B*H*S float32 rows (16 MiB per GPU). */
 #define FA_NOALLOC_MAX_ROWS (1 << 22)
 
-enum fa_dtype { FA_DTYPE_F16 = 0, FA_DTYPE_BF16 = 1 };
+enum fa_dtype { FA_DTYPE_F16 = 0, FA_DTYPE_BF16 = 1, FA_DTYPE_F32 = 2 /* norm weights only */ };
 
 /* ABI version of the loaded library (FA_ABI_VERSION at build time). */
 FA_API int fa_abi_version(void);
@@ -117,6 +117,89 @@ FA_API int fa_bwd_noalloc(const void* q, const void* k, const void* v, const voi
                           const void* dO, const float* lse, void* dq, void* dk, void* dv,
                           int B, int H, int H_kv, int S, int D, int dtype, int tile_m, int tile_n,
                           int* dev_status, void* stream);
+
+/* ---- Around attention: norm + rotary positions, the paged e4m3 cache, attention over it ----
+ * No counterpart in the reference.  Arguments travel in one struct; the rules at the top of this
+ * file hold.  16-bit rows are contiguous in D and start on 16-byte boundaries: base addresses are
+ * 16-byte aligned and strides (in elements) multiples of 8.  A position, page, sequence length or
+ * offset that lies outside its table is found by the kernel: it records code 111 in dev_status[0]
+ * and stays inside its buffers; what the call wrote is then undefined. */
+
+/* Rows of float32 [D] that fa_norm_rope_bwd's workspace holds. */
+#define FA_ROPE_WORKSPACE_ROWS 296
+
+/* z = rotate(norm(x)) for every row x of q and k (k may be NULL with H_kv = 0):
+ *   norm(x)[d] = x[d] * w[d] / sqrt(mean(x^2) + eps), the identity where the weight is NULL;
+ *   rotate turns pair i, (x[i], x[i + D/2]) or interleaved (x[2i], x[2i+1]), by the angle whose
+ *   cosine and sine stand in row p of cos and sin, p the token's position on the pair's axis.
+ * Axis a has the pairs [section_start[a], section_start[a + 1]); section_start[0] = 0.
+ * Forward writes q_out and k_out (contiguous [B, H, N, D]).  Backward reads q, k and dq_out, dk_out
+ * (contiguous), writes dq, dk, and dq_weight, dk_weight [D] (type of the weights) where not NULL,
+ * through workspace, FA_ROPE_WORKSPACE_ROWS * D floats; two runs give the same bits. */
+struct fa_norm_rope_args {
+  const void *q, *k, *q_weight, *k_weight;
+  const float *cos, *sin;      /* [max_pos, D/2] */
+  const void* pos;             /* position of (axis, b, n): pos[axis * pos_stride[0] + b * pos_stride[1] + n];
+                                  NULL: n */
+  void *q_out, *k_out;
+  const void *dq_out, *dk_out;
+  void *dq, *dk, *dq_weight, *dk_weight;
+  float* workspace;
+  long long q_stride[3], k_stride[3], dq_stride[3], dk_stride[3]; /* batch, head, token */
+  long long pos_stride[2];
+  int B, H, H_kv, N, D, dtype, weight_dtype, max_pos, axes;
+  int section_start[4];
+  int pos_is_int64, interleaved;
+  float eps;
+};
+FA_API int fa_norm_rope_fwd(const struct fa_norm_rope_args* args, int* dev_status, void* stream);
+FA_API int fa_norm_rope_bwd(const struct fa_norm_rope_args* args, int* dev_status, void* stream);
+
+/* Appends T new tokens' keys and values ([T, H_kv, D]) to a cache of e4m3 pages [num_pages, H_kv,
+ * page_size, D] with float32 scales [num_pages, H_kv]; a byte c stands for float(c) * scale.
+ * Sequence b's new tokens are offsets[b] .. offsets[b + 1] (offsets NULL: token b, T = B); they are
+ * the last of its seq_lens[b] tokens, and token j lies in page block_table[b][j / page_size].
+ * Keys are normed and rotated like above where k_weight / cos are given (pos NULL: the position is
+ * j).  The scale of a page is the smallest power of two that holds its tokens of this call in
+ * +-448, and not less than before where the page holds older tokens (those are rounded again when
+ * it grows).  Tokens at j < 0 and tokens behind offsets[B] are left out.  A page that is written
+ * must belong to one sequence.  page_size in {16, 32, 64, 128}. */
+struct fa_append_args {
+  const void *k, *v;
+  void *k_pages, *v_pages;
+  float *k_scales, *v_scales;
+  const int *block_table, *seq_lens, *offsets;
+  const float *cos, *sin;
+  const void *pos, *k_weight;
+  long long k_stride[2], v_stride[2]; /* token, head */
+  long long table_stride, pos_axis_stride;
+  double eps;
+  int T, B, width, num_pages, H_kv, page_size, D, dtype, weight_dtype, max_pos, axes;
+  int section_start[4];
+  int pos_is_int64, interleaved, reserved;
+};
+FA_API int fa_append_kv(const struct fa_append_args* args, int* dev_status, void* stream);
+
+/* Bytes of workspace that fa_paged_attention needs for head dim D. */
+#define FA_PAGED_WORKSPACE_BYTES(D) (40960LL * (D) + 131072)
+
+/* Attention of T query tokens ([T, H, D]) over the cache: query token i of sequence b's n new tokens
+ * sees its keys j <= seq_lens[b] - n + i.  out [T, H, D]; lse [T, H] (log2 domain) or NULL; a row
+ * that sees no key gets 0 and -inf.  Tokens behind offsets[B] are left as they are. */
+struct fa_paged_args {
+  const void* q;
+  const void *k_pages, *v_pages;
+  const float *k_scales, *v_scales;
+  const int *block_table, *seq_lens, *offsets;
+  void* out;
+  float* lse;
+  void* workspace;             /* FA_PAGED_WORKSPACE_BYTES(D), 16-byte aligned; not shared by calls that overlap */
+  long long q_stride[2], out_stride[2]; /* token, head */
+  long long table_stride;
+  int T, B, width, num_pages, H, H_kv, page_size, D, dtype;
+  float scale;
+};
+FA_API int fa_paged_attention(const struct fa_paged_args* args, int* dev_status, void* stream);
 
 #ifdef __cplusplus
 }
