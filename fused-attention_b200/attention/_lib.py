@@ -11,13 +11,14 @@ reference's `ct.launch(torch.cuda.current_stream(), ...)` (attention/fused/fused
 """
 import contextlib
 import ctypes
+import importlib.util
 import os
-import struct
 import threading
 
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfa_sm100.so")
+OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_fa_torch.so")
 ABI_VERSION = 2
 
 
@@ -220,57 +221,33 @@ def unfused_fwd(q, k, v, o, s, p):
                                     p.data_ptr(), B, H, k.shape[1], S, D, _dtype_code(q)))])
 
 
-# ---- norm + rotary positions, paged cache, attention over it: arguments travel in one struct
-# (include/fa_sm100.h); a packed bytes object converts to its pointer.
-NORM_ROPE_ARGS = struct.Struct("@16P14q15if")
-APPEND_ARGS = struct.Struct("@13P6qd18i")
-PAGED_ARGS = struct.Struct("@11P5q9if")
-ROPE_WORKSPACE_ROWS = 296
-F32_CODE = 2
+_ops = None
 
 
-def paged_workspace_bytes(head_dim):
-    return 40960 * head_dim + 131072
+def _status_for_ops(idx, only_ask):
+    """The status word of device idx for the native torch binding: its address, or whether it is there."""
+    if only_ask:
+        return idx in _status
+    return status_tensor(torch.device("cuda", idx)).data_ptr()
 
 
-def norm_rope_fwd(q, packed):
-    _launch(q, [("fa_norm_rope_fwd", (packed,))])
-
-
-def norm_rope_bwd(q, packed):
-    _launch(q, [("fa_norm_rope_bwd", (packed,))])
-
-
-def append_kv(k, packed):
-    _launch(k, [("fa_append_kv", (packed,))])
-
-
-def paged_attention(q, packed):
-    _launch(q, [("fa_paged_attention", (packed,))])
-
-
-def rows16(x):
-    """x as the kernels take 16-bit rows: contiguous in its last dimension, base and strides on 16-byte
-    boundaries (a copy where it is not), and its other strides (0 for dimensions of size 1)."""
-    size, stride = x.shape, x.stride()
-    ok = stride[-1] == 1 and x.data_ptr() % 16 == 0
-    strides = []
-    for n, s in zip(size[:-1], stride[:-1]):
-        if n == 1:
-            s = 0
-        elif s % 8 or s < 0:
-            ok = False
-        strides.append(s)
-    if ok:
-        return x, strides
-    x = x.clone(memory_format=torch.contiguous_format)
-    return x, [0 if n == 1 else s for n, s in zip(x.shape[:-1], x.stride()[:-1])]
-
-
-def aligned16(x):
-    """x contiguous with its base on a 16-byte boundary (a copy where it is not)."""
-    x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
+def load_ops():
+    """Load (once) and return the native torch binding (csrc/fa_torch.cpp) of the operators around
+    attention: it checks the tensors, allocates outputs and calls the C ABI."""
+    global _ops
+    if _ops is not None:
+        return _ops
+    load()
+    with _lock:
+        if _ops is None:
+            if not os.path.exists(OPS_PATH):
+                raise RuntimeError(f"{OPS_PATH} is not built; run `python fused-attention_b200/build.py`")
+            spec = importlib.util.spec_from_file_location("_fa_torch", OPS_PATH)
+            ops = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(ops)
+            ops.set_status_provider(_status_for_ops)
+            _ops = ops
+    return _ops
 
 
 def load_by_path():

@@ -4,6 +4,9 @@
     python fused-attention_b200/build.py --force    # rebuild everything
     python fused-attention_b200/build.py --verbose  # also print ptxas register/smem usage
 
+build_ops() compiles csrc/fa_torch.cpp, the native torch binding of the operators around attention, into
+attention/_fa_torch.so against the installed torch; it links libfa_sm100.so next to it.
+
 The shared library lands next to the Python package (attention/libfa_sm100.so), so it travels
 with the source tree.  Objects go to _build/ (not committed).
 
@@ -17,12 +20,14 @@ import argparse
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "attention", "libfa_sm100.so")
+OPS_OUT = os.path.join(HERE, "attention", "_fa_torch.so")
 STALL_OUT = os.path.join(BUILD, "libfa_sm100_stalltest.so")
 STALL_FLAGS = ["-DFA_TEST_STALL_STEP=1", "-DFA_WAIT_TIMEOUT_NS=20000000ull"]
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
@@ -80,6 +85,28 @@ def build(force=False, verbose=False, out=OUT, extra_flags=(), obj_dir=BUILD):
     return out
 
 
+def build_ops(force=False, out=OPS_OUT):
+    """The native torch binding (see the module docstring); libfa_sm100.so must be built."""
+    src = os.path.join(CSRC, "fa_torch.cpp")
+    if not force and not _newer([src, os.path.join(INCLUDE, "fa_sm100.h")], out):
+        return out
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    include = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], INCLUDE]
+    # the C++ runtime is named as a shared library: torch's is, and a second, static one crashes in its streams
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-DTORCH_EXTENSION_NAME=_fa_torch", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(x for d in include for x in ("-isystem", d)), src, "-o", out, "-l:libstdc++.so.6", f"-L{os.path.dirname(OUT)}", "-l:libfa_sm100.so",
+           "-Wl,-rpath,$ORIGIN", f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10",
+           "-lc10_cuda", "-ltorch_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed")
+    return out
+
+
 def build_stall_test(force=False, verbose=False):
     """The failure-detection test library (see the module docstring)."""
     return build(force, verbose, out=STALL_OUT, extra_flags=STALL_FLAGS,
@@ -92,4 +119,5 @@ if __name__ == "__main__":
     ap.add_argument("--verbose", action="store_true")
     a = ap.parse_args()
     print(build(force=a.force, verbose=a.verbose))
+    print(build_ops(force=a.force))
     print(build_stall_test(force=a.force))
