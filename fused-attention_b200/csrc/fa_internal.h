@@ -152,7 +152,8 @@ struct PagedParams {
   long long out_stride[2];
   long long table_stride;
   int* status;
-  int T, B, num_pages, H_kv, group, page_size;
+  int T, B, num_pages, H_kv, group;
+  int page_shift;            // log2(page size)
   int capacity;              // tokens that a row of the table can name
   int bf16;
   float scale_log2;          // log2(e) * softmax scale
@@ -203,7 +204,7 @@ cudaError_t launch_rope_bwd(RopeParams p, int D, bool bf16, bool interleaved, cu
 
 cudaError_t launch_append(AppendParams p, int D, bool bf16, bool interleaved, cudaStream_t stream);
 int paged_row_tile(const PagedParams& p);
-int paged_blocks(const PagedParams& p);  // size of the split kernel's grid
+int paged_blocks(const PagedParams& p, int D);  // size of the split kernel's grid
 cudaError_t launch_paged(const PagedParams& p, int D, int blocks, cudaStream_t stream);
 
 // Launchers implemented in the kernel translation units.  They return a cudaError_t.

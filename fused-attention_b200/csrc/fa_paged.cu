@@ -16,14 +16,17 @@
 //     softmax state, and are joined in shared memory once per tile of rows.
 //   * Matrix form.  S^T = K Q^T and O^T = V^T P^T on m16n8k16 (f16 in, f32 sums): keys (and for
 //     O^T the head dim) are the 16-row side, query rows the 8-column side, so a group of 8 heads
-//     wastes nothing.  The 16-row operands come straight from global memory into registers: the
-//     k index of S^T (the head dim) and the m index of O^T (again the head dim) may be permuted
-//     freely, which lets a thread take 16-byte pieces of a cached row.  S^T leaves the
-//     instruction as an 8 x 8 tile whose transpose is the second product's operand (movmatrix).
+//     wastes nothing.  The k index of S^T (the head dim) and the m index of O^T (again the head
+//     dim) may be permuted freely, which lets a thread take 16-byte pieces of a cached row and turn
+//     bytes into operands with one conversion per pair.  S^T leaves the instruction as an 8 x 8 tile
+//     whose transpose is the second product's operand (movmatrix).  The e4m3 form of mma.sync would
+//     spare the conversions, but it is not a machine instruction here (it expands into conversions and
+//     f16 products; measured 74 us instead of 68 for 32 sequences of up to 8192).
 //   * Types.  e4m3 is exact in f16, so K and V lose nothing; bf16 queries are brought into f16's
-//     range by a power of two per row (exact).  P is f16 relative to a running maximum of
-//     s + log2(v_scale), so the pages' scales ride in P's exponent and a page with a small scale
-//     loses no precision; the softmax sum uses its own maximum, per thread, in float32.
+//     range by a power of two per row (exact).  P is f16 relative to a reference of s +
+//     log2(v_scale), so the pages' scales ride in P's exponent and a page with a small scale loses no
+//     precision; the softmax sum has its own reference, per thread, in float32.  A reference moves
+//     only when a score passes it by 2^kSlack: O is rescaled, and lanes compare notes, only then.
 //   K of the next tile is loaded before the softmax of this one, V of this one before its S.
 #include "fa_internal.h"
 #include "fa_sm100.cuh"
@@ -37,6 +40,12 @@ constexpr int kPagedThreads = 128;
 constexpr int kWarps = kPagedThreads / 32;
 constexpr int kUnit = kPagedUnit;   // keys of a unit
 constexpr int kTile = 32;           // keys of a warp's tile
+constexpr float kSlack = 8.f;       // log2: weights stay below 2^8 of the reference, far inside f16
+
+template <int D, int NT>
+struct PagedCfg {  // resident blocks per SM, as the registers allow
+  static constexpr int kPerSm = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
+};
 
 // Two e4m3 bytes (the low 16 bits of v) -> two f16.
 __device__ __forceinline__ uint32_t cvt2(uint32_t v) {
@@ -52,7 +61,7 @@ __device__ __forceinline__ uint32_t cvt2_hi(uint32_t v) {
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -219,8 +228,8 @@ struct RowTile {
 template <int D, int NT>
 struct WarpState {
   float o[NT][D / 16][4];   // O^T: rows g, g + 8 of each 16-row tile, columns 2t, 2t + 1
-  float mw[NT][2];          // running maximum of s + log2(v_scale), all lanes of a column alike
-  float m[NT][2];           // this thread's running maximum of s
+  float mw[NT][2];          // reference of s + log2(v_scale), all lanes of a column alike
+  float m[NT][2];           // this thread's reference of s
   float l[NT][2];           // this thread's sum of 2^(s - m)
 };
 
@@ -228,51 +237,70 @@ template <int D, int NT, bool EDGE>
 __device__ __forceinline__ void softmax_pv(WarpState<D, NT>& st, float (&s)[NT][2][4], const float (&qs)[NT][2],
                                            const float (&ks)[2], const float (&vs)[2], VBlock<D> (&v)[2],
                                            const int (&last)[NT][2], int key0, int keys, int g, int t) {
-  uint32_t pb[NT][2][2];
+  bool raise = false;
+  float top[NT][2][2];  // per column: this thread's largest score, and with its page's scale
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      // the column's four scores of this thread: blocks 0, 1, rows g, g + 8
-      float tm = -INFINITY, tw = -INFINITY;
+      float block_top[2];
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
+      for (int blk = 0; blk < 2; ++blk) {
+        const float f = qs[nt][c] * ks[blk];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float x = s[nt][blk][2 * r + c] * (qs[nt][c] * ks[blk]);
+          float x = s[nt][blk][2 * r + c] * f;
           if (EDGE && key0 + 16 * blk + 8 * r + g > last[nt][c]) x = -INFINITY;
           s[nt][blk][2 * r + c] = x;
-          tm = fmaxf(tm, x);
-          tw = fmaxf(tw, x + vs[blk]);
         }
+        block_top[blk] = fmaxf(s[nt][blk][c], s[nt][blk][2 + c]);
+      }
+      top[nt][c][0] = fmaxf(block_top[0], block_top[1]);
+      top[nt][c][1] = fmaxf(block_top[0] + vs[0], block_top[1] + vs[1]);
+      raise |= top[nt][c][1] > st.mw[nt][c] + kSlack;
+    }
+  if (__any_sync(0xffffffffu, raise)) {  // new references, the same in all lanes of a column
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) tw = fmaxf(tw, __shfl_xor_sync(0xffffffffu, tw, o));
-      const float old_w = st.mw[nt][c];
-      const float new_w = fmaxf(old_w, tw);
-      const float ref_w = new_w == -INFINITY ? 0.f : new_w;
-      const float alpha = ex2_approx(old_w - ref_w);
-      st.mw[nt][c] = new_w;
-      const float old_m = st.m[nt][c];
-      const float new_m = fmaxf(old_m, tm);
-      const float ref_m = new_m == -INFINITY ? 0.f : new_m;
-      st.m[nt][c] = new_m;
-      float l = st.l[nt][c] * ex2_approx(old_m - ref_m);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
+      for (int c = 0; c < 2; ++c) {
+        float ref = top[nt][c][1];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float x = s[nt][blk][2 * r + c];
-          l += ex2_approx(x - ref_m);
-          s[nt][blk][2 * r + c] = ex2_approx(x + vs[blk] - ref_w);
-        }
-      st.l[nt][c] = l;
-      if (alpha != 1.f) {
+        for (int o = 4; o < 32; o <<= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+        ref = fmaxf(st.mw[nt][c], ref);
+        const float alpha = st.mw[nt][c] == -INFINITY ? 0.f : ex2_approx(st.mw[nt][c] - ref);
+        st.mw[nt][c] = ref;
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt) {
           st.o[nt][mt][c] *= alpha;
           st.o[nt][mt][2 + c] *= alpha;
         }
       }
+  }
+  uint32_t pb[NT][2][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float m = st.m[nt][c], l = st.l[nt][c];
+      if (top[nt][c][0] > m + kSlack) {  // also the first score of the thread (m = -inf, l = 0)
+        l = m == -INFINITY ? 0.f : l * ex2_approx(m - top[nt][c][0]);
+        m = top[nt][c][0];
+        st.m[nt][c] = m;
+      }
+      const float rm = m == -INFINITY ? 0.f : m;  // no score yet: all terms below are 0
+      const float rw = st.mw[nt][c] == -INFINITY ? 0.f : st.mw[nt][c];
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        const float rb = rw - vs[blk];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float x = s[nt][blk][2 * r + c];
+          l += ex2_approx(x - rm);
+          s[nt][blk][2 * r + c] = ex2_approx(x - rb);
+        }
+      }
+      st.l[nt][c] = l;
     }
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk)
@@ -305,7 +333,7 @@ __device__ __forceinline__ void softmax_pv(WarpState<D, NT>& st, float (&s)[NT][
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 3 : 2) paged_split_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_split_kernel(const PagedParams p) {
   constexpr int RT = 8 * NT;
   __shared__ float sh_o[kWarps][RT][D + 4];  // +4: rows start on different banks
   __shared__ float sh_m[kWarps][RT], sh_l[kWarps][RT];
@@ -322,7 +350,8 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 3 : 2) paged_split_ke
   if (static_cast<long long>(blockIdx.x) >= blocks) return;
   long long unit = cur.total * blockIdx.x / blocks;
   const long long unit_end = cur.total * (blockIdx.x + 1) / blocks;
-  const uint32_t kv_head_bytes = static_cast<uint32_t>(p.page_size) * D;
+  const uint32_t kv_head_bytes = static_cast<uint32_t>(D) << p.page_shift;
+  const int page_mask = (1 << p.page_shift) - 1;
   int b = cur.b;
   long long skip = cur.skip;
   bool first_segment = true;
@@ -409,10 +438,10 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 3 : 2) paged_split_ke
     // ---- this warp's 32-key tiles of keys [u0, u1) units
     const int key_end = min(keys, u1 * kUnit);
     const int* table = p.block_table + b * p.table_stride;
-    const int last_index = keys > 0 ? (keys - 1) / p.page_size : 0;
+    const int last_index = keys > 0 ? (keys - 1) >> p.page_shift : 0;
     // The page of a 16-key block; blocks behind the last key stay on its page.
     auto page_of = [&](int key) -> int {
-      const int page = table[min(key / p.page_size, last_index)];
+      const int page = table[min(key >> p.page_shift, last_index)];
       if (page < 0 || page >= p.num_pages) {
         record_error(p.status, kDevBadIndex, b);
         return 0;
@@ -429,7 +458,7 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 3 : 2) paged_split_ke
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
         at[blk] = static_cast<size_t>(next_page[blk]) * p.H_kv + h;
-        load_k<D>(p.k_pages + at[blk] * kv_head_bytes + (key0 + 16 * blk) % p.page_size * D, g, t, k[blk]);
+        load_k<D>(p.k_pages + at[blk] * kv_head_bytes + ((key0 + 16 * blk) & page_mask) * D, g, t, k[blk]);
       }
       int key_next = key0 + kWarps * kTile;
       if (key_next < key_end)
@@ -440,7 +469,7 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 3 : 2) paged_split_ke
         float ks[2], vs[2];
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
-          load_v<D>(p.v_pages + at[blk] * kv_head_bytes + (key0 + 16 * blk) % p.page_size * D, g, t, v[blk]);
+          load_v<D>(p.v_pages + at[blk] * kv_head_bytes + ((key0 + 16 * blk) & page_mask) * D, g, t, v[blk]);
           ks[blk] = p.k_scales[at[blk]];
           vs[blk] = p.v_scales[at[blk]];
         }
@@ -465,14 +494,14 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 3 : 2) paged_split_ke
 #pragma unroll
           for (int blk = 0; blk < 2; ++blk) {
             at[blk] = static_cast<size_t>(next_page[blk]) * p.H_kv + h;
-            load_k<D>(p.k_pages + at[blk] * kv_head_bytes + (key_next + 16 * blk) % p.page_size * D, g, t, k[blk]);
+            load_k<D>(p.k_pages + at[blk] * kv_head_bytes + ((key_next + 16 * blk) & page_mask) * D, g, t, k[blk]);
           }
           if (key_next + kWarps * kTile < key_end)
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) next_page[blk] = page_of(key_next + kWarps * kTile + 16 * blk);
         }
-        vs[0] = log2f(vs[0]);
-        vs[1] = log2f(vs[1]);
+        vs[0] = __log2f(vs[0]);
+        vs[1] = __log2f(vs[1]);
         if (key0 + kTile > seen_by_all)
           softmax_pv<D, NT, true>(st, s, qs, ks, vs, v, last, key0, keys, g, t);
         else
@@ -583,70 +612,76 @@ constexpr int kJoinSplit = kJoinThreads / 32 / kJoinRows;
 template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedParams p) {
   constexpr int RT = 8 * NT;
-  constexpr int V = D / 32;  // values of a lane
+  constexpr int V = D / 32;  // consecutive values of a lane
   __shared__ float sh_o[kJoinRows][kJoinSplit][D];
-  __shared__ float sh_m[kJoinRows][kJoinSplit], sh_l[kJoinRows][kJoinSplit];
+  __shared__ float sh_l[kJoinRows][kJoinSplit];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PagedJoin j = p.joins[blockIdx.x];
   if (j.parts == 0) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int local = warp / kJoinSplit, split = warp % kJoinSplit;
   const int r = blockIdx.y * kJoinRows + local;
-  float m = -INFINITY, l = 0.f, acc[V];
+  const bool live = r < j.rows;
+  auto slot_of = [&](int i) -> size_t { return i == 0 ? j.slot : 2 * (blockIdx.x + static_cast<size_t>(i)); };
+  // the row's maximum over all parts first: the parts can then be loaded without waiting for each other
+  float m = -INFINITY;
+  if (live)
+    for (int i = lane; i < j.parts; i += 32) m = fmaxf(m, p.part_ml[slot_of(i) * RT + r].x);
 #pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  if (r < j.rows) {
-#pragma unroll 4
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  if (live) {
+#pragma unroll 8
     for (int i = split; i < j.parts; i += kJoinSplit) {
-      const size_t slot = i == 0 ? j.slot : 2 * (blockIdx.x + static_cast<size_t>(i));
-      const float2 ml = p.part_ml[slot * RT + r];
-      const float* o = p.parts + (slot * RT + r) * D + lane;
+      const size_t at = slot_of(i) * RT + r;
+      const float2 ml = p.part_ml[at];
+      const float* o = p.parts + at * D + V * lane;
       float x[V];
+      if constexpr (V == 4) {
+        const float4 q = *reinterpret_cast<const float4*>(o);
+        x[0] = q.x;
+        x[1] = q.y;
+        x[2] = q.z;
+        x[3] = q.w;
+      } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = o[32 * v];
-      const float nm = fmaxf(m, ml.x);
-      const float ref = nm == -INFINITY ? 0.f : nm;
-      const float a = ex2_approx(m - ref), f = ex2_approx(ml.x - ref);
-      l = l * a + ml.y * f;
+        for (int v = 0; v < V; ++v) x[v] = o[v];
+      }
+      const float f = ex2_approx(ml.x - ref);
+      l = fmaf(ml.y, f, l);
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = acc[v] * a + x[v] * f;
-      m = nm;
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(x[v], f, acc[v]);
     }
   }
 #pragma unroll
-  for (int v = 0; v < V; ++v) sh_o[local][split][lane + 32 * v] = acc[v];
-  if (lane == 0) {
-    sh_m[local][split] = m;
-    sh_l[local][split] = l;
-  }
+  for (int v = 0; v < V; ++v) sh_o[local][split][V * lane + v] = acc[v];
+  if (lane == 0) sh_l[local][split] = l;
   __syncthreads();
-  if (split != 0 || r >= j.rows) return;
-  m = sh_m[local][0];
-#pragma unroll
-  for (int s = 1; s < kJoinSplit; ++s) m = fmaxf(m, sh_m[local][s]);
-  const float ref = m == -INFINITY ? 0.f : m;
+  if (split != 0 || !live) return;
   l = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.f;
 #pragma unroll
   for (int s = 0; s < kJoinSplit; ++s) {
-    const float f = ex2_approx(sh_m[local][s] - ref);
-    l += sh_l[local][s] * f;
+    l += sh_l[local][s];
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] += sh_o[local][s][lane + 32 * v] * f;
+    for (int v = 0; v < V; ++v) acc[v] += sh_o[local][s][V * lane + v];
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const int row = j.row + r;
   const long long token = j.token + row / p.group;
   const int head = j.head * p.group + row % p.group;
-  const long long at = token * p.out_stride[0] + head * p.out_stride[1];
+  const long long at = token * p.out_stride[0] + head * p.out_stride[1] + V * lane;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const float x = acc[v] * inv;
     if (p.bf16)
-      static_cast<__nv_bfloat16*>(p.out)[at + lane + 32 * v] = __float2bfloat16_rn(x);
+      static_cast<__nv_bfloat16*>(p.out)[at + v] = __float2bfloat16_rn(x);
     else
-      static_cast<__half*>(p.out)[at + lane + 32 * v] = __float2half_rn(x);
+      static_cast<__half*>(p.out)[at + v] = __float2half_rn(x);
   }
   if (p.lse != nullptr && lane == 0)
     p.lse[token * p.group * p.H_kv + head] = l == 0.f ? -INFINITY : m + log2f(l);
@@ -670,6 +705,11 @@ cudaError_t launch_paged_t(const PagedParams& p, int blocks, bool join, cudaStre
   return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, NT>, p);
 }
 
+int resident_blocks(int D, int row_tile) {
+  if (D == 128) return row_tile == 8 ? PagedCfg<128, 1>::kPerSm : PagedCfg<128, 2>::kPerSm;
+  return row_tile == 8 ? PagedCfg<64, 1>::kPerSm : PagedCfg<64, 2>::kPerSm;
+}
+
 }  // namespace
 
 int paged_row_tile(const PagedParams& p) {
@@ -678,9 +718,9 @@ int paged_row_tile(const PagedParams& p) {
   return rows <= 8LL * p.B ? 8 : 16;
 }
 
-int paged_blocks(const PagedParams& p) {
+int paged_blocks(const PagedParams& p, int D) {
   const int row_tile = paged_row_tile(p);
-  const int resident = row_tile == 8 ? 3 : 2;  // blocks per SM
+  const int resident = resident_blocks(D, row_tile);  // blocks per SM
   const long long tiles = (static_cast<long long>(p.T) * p.group + row_tile - 1) / row_tile + p.B;
   const long long units = tiles * p.H_kv * ((p.capacity + kUnit - 1) / kUnit);
   return static_cast<int>(units < 148 * resident ? units : 148 * resident);

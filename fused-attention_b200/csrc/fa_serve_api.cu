@@ -221,11 +221,11 @@ int fa_paged_attention(const fa_paged_args* a, int* dev_status, void* stream) {
   p.num_pages = a->num_pages;
   p.H_kv = a->H_kv;
   p.group = a->H / a->H_kv;
-  p.page_size = a->page_size;
+  p.page_shift = a->page_size == 16 ? 4 : (a->page_size == 32 ? 5 : (a->page_size == 64 ? 6 : 7));
   p.capacity = a->width * a->page_size;
   p.bf16 = a->dtype == FA_DTYPE_BF16;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  const int blocks = fa::paged_blocks(p);
+  const int blocks = fa::paged_blocks(p, a->D);
   const size_t rows = 2 * static_cast<size_t>(blocks) * fa::paged_row_tile(p);
   p.joins = static_cast<fa::PagedJoin*>(a->workspace);  // 24 bytes each, then 16-byte aligned arrays
   uint8_t* at = static_cast<uint8_t*>(a->workspace) + (blocks * sizeof(fa::PagedJoin) + 15) / 16 * 16;

@@ -208,8 +208,10 @@ Tensor empty_like_rows(const Tensor& x) {
 }
 
 struct NormRope : torch::autograd::Function<NormRope> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
-                                                const Tensor& qw, const Tensor& kw, const Turn& t, double eps, bool interleaved) {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k_opt,
+                                                const OptTensor& qw_opt, const OptTensor& kw_opt, const Turn& t, double eps,
+                                                bool interleaved) {
+    const Tensor k = k_opt.value_or(Tensor()), qw = qw_opt.value_or(Tensor()), kw = kw_opt.value_or(Tensor());
     ctx->save_for_backward({q, k, qw, kw, t.cos, t.sin, t.pos});
     ctx->saved_data["turn"] = std::vector<int64_t>{t.start[0], t.start[1], t.start[2], t.start[3], t.axes, t.pos_stride[0],
                                                    t.pos_stride[1], interleaved};
@@ -232,7 +234,9 @@ struct NormRope : torch::autograd::Function<NormRope> {
     t.axes = static_cast<int>(v[4]);
     t.pos_stride[0] = v[5];
     t.pos_stride[1] = v[6];
-    const bool want_qw = ctx->needs_input_grad(2), want_kw = ctx->needs_input_grad(3);
+    // gradients are asked for by the place among the tensors that were given
+    const size_t at_qw = k.defined() ? 2 : 1, at_kw = at_qw + (qw.defined() ? 1 : 0);
+    const bool want_qw = qw.defined() && ctx->needs_input_grad(at_qw), want_kw = kw.defined() && ctx->needs_input_grad(at_kw);
     if (q.numel() == 0)
       return {at::zeros_like(q), k.defined() ? at::zeros_like(k) : Tensor(), want_qw ? at::zeros_like(qw) : Tensor(),
               want_kw ? at::zeros_like(kw) : Tensor(), Tensor(), Tensor(), Tensor()};
@@ -294,7 +298,7 @@ std::pair<Tensor, OptTensor> qk_norm_rope(const Tensor& q, const OptTensor& k_op
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()) ||
                                                    (qw.defined() && qw.requires_grad()) || (kw.defined() && kw.requires_grad()));
   if (grad) {
-    const auto out = NormRope::apply(q, k, qw, kw, t, eps, interleaved);
+    const auto out = NormRope::apply(q, k_opt, q_weight, k_weight, t, eps, interleaved);
     return {out[0], k.defined() ? OptTensor(out[1]) : std::nullopt};
   }
   const auto [q_out, k_out] = rope_forward(q, k, qw, kw, t, eps, interleaved);

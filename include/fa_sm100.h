@@ -181,7 +181,7 @@ struct fa_append_args {
 FA_API int fa_append_kv(const struct fa_append_args* args, int* dev_status, void* stream);
 
 /* Bytes of workspace that fa_paged_attention needs for head dim D. */
-#define FA_PAGED_WORKSPACE_BYTES(D) (40960LL * (D) + 131072)
+#define FA_PAGED_WORKSPACE_BYTES(D) (75776LL * (D) + 196608)
 
 /* Attention of T query tokens ([T, H, D]) over the cache: query token i of sequence b's n new tokens
  * sees its keys j <= seq_lens[b] - n + i.  out [T, H, D]; lse [T, H] (log2 domain) or NULL; a row
