@@ -1,0 +1,634 @@
+// Attention over a paged e4m3 cache for many query rows (prompts in chunks behind what is cached), for
+// sm_100a: tcgen05 UMMA on f16 tiles that a warpgroup makes from the cached bytes.
+//
+//   s_j = (q . k8_j) * k_scale(page j) * scale,   o = sum_j softmax(s)_j * v_scale(page j) * v8_j
+// Token i of a sequence's n new tokens, at sequence length L, sees keys j <= L - n + i.
+//
+// Bound: the tensor cores and the exponentials, as in the dense forward (fa_fwd.cu), whose structure
+// this is: a block owns two 128-row query tiles that read the same K/V head, one thread per row.  Here
+//   * rows are (token, head of the group) pairs, so a tile of a group of G heads covers 128 / G tokens and
+//     every cached byte a block reads serves 256 rows;
+//   * K and V tiles are built by a warpgroup of their own: 16-byte pieces of a page, e4m3 -> f16 (exact),
+//     times the page's scale, into the swizzled layout that the tensor core reads.  The scale is taken
+//     relative to the sequence's largest, ref: f16(64 v8 scale / ref) is exact for power-of-two scales
+//     down to 2^-21 of the largest (below, values keep an absolute precision of 2^-40 of the largest page's
+//     magnitude; scales that are no powers of two are rounded to f16's 11 bits).  So S and O need no
+//     per-page arithmetic, and the 64 keys-by-key conversions cost the softmax warps nothing;
+//   * queries are brought to f16 by a power of two per row (exact down to 2^-31 of the row's largest
+//     element) by the thread that owns the row; P is f16.
+// Warp roles (512 threads):
+//   warps 0-3, 4-7  softmax warpgroups of query tiles 0 and 1 (they load Q and write O)
+//   warp 8          UMMA issuer: S_t = Q_t K_j^T, O_t += P_t V_j with P_t in TMEM
+//   warps 9-11      idle
+//   warps 12-15     K and V tiles
+// Registers: 128 a thread at launch; warps 8-15 drop to kRegsOther, the softmax warps rise to
+// kRegsSoftmax, and 256 x kRegsOther + 256 x kRegsSoftmax = 512 x 128.
+// TMEM (512 columns): S_0 | S_1 | O_0 | O_1, P_t over the first half of S_t; P is published in two halves.
+#include "fa_internal.h"
+#include "fa_sm100.cuh"
+#include "fa_softmax.cuh"
+
+#include <cuda_fp8.h>
+
+namespace fa {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kWarpMma = 8;
+constexpr int kWarpTiles = 12;  // first of the four warps that build K and V tiles
+constexpr int kBM = 128;
+constexpr int kBN = 128;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr int kLaunchRegs = 128;
+constexpr int kRegsSoftmax = 192;
+constexpr int kRegsOther = 64;
+static_assert(256 * kRegsOther + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split");
+constexpr int kSoftmaxCopy = 1;  // the softmax warpgroups' own copy of the bounded-wait loop
+constexpr int kPolyPairs = 4;    // of 16 exp2 pairs on interior tiles: the dense forward's share
+constexpr float kHeadroom = 64.f;  // f16(448 * 64) is finite
+
+template <int D>
+struct ChunkCfg {
+  static constexpr int kSwBytes = D >= 64 ? 128 : 64;  // a shared-memory row: one swizzle span
+  static constexpr uint32_t kLayout = D >= 64 ? kLayoutSw128 : kLayoutSw64;
+  static constexpr int kSbo = 8 * kSwBytes;
+  static constexpr int kKStepsPerChunk = kSwBytes / 32;
+  static constexpr int kChunkBytes = 128 * kSwBytes;   // Q, K and V tiles all have 128 rows
+  static constexpr int kTileBytes = 128 * D * 2;
+  static constexpr int kStages = D == 128 ? 2 : 4;     // K and V rings
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = 2 * kTileBytes;
+  static constexpr int kOffV = kOffK + kStages * kTileBytes;
+  static constexpr int kOffBar = kOffV + kStages * kTileBytes;
+  static constexpr int kSmemBytes = kOffBar + 512 + 1024;  // barriers, scan words, alignment slack
+  // Byte offset of 16-byte piece c of row r of an f16 tile (pieces of D / 8 per row).
+  static __device__ __forceinline__ uint32_t place(int r, int c) {
+    if constexpr (D >= 64) return (c >> 3) * kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+  }
+};
+
+enum : int {
+  BAR_Q = 0,        // + tile (2)
+  BAR_KFULL = 2,    // + stage (4)
+  BAR_KEMPTY = 6,
+  BAR_VFULL = 10,
+  BAR_VEMPTY = 14,
+  BAR_SFULL = 18,   // + tile (2)
+  BAR_PFULLA = 20,
+  BAR_PFULLB = 22,
+  BAR_OFULL = 24,
+  BAR_DRAIN = 26,
+  BAR_NEVER = 27,   // never arrived at (the failure-detection test build waits on it)
+  BAR_COUNT = 28
+};
+
+// One 16-byte piece of a cached row -> 16 f16 values times f.
+__device__ __forceinline__ void dequant16(const uint4& raw, uint32_t f, uint4& lo, uint4& hi) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t h[8];
+  const __half2 scale = *reinterpret_cast<const __half2*>(&f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t a, b;
+    asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+        : "=r"(a), "=r"(b) : "r"(w[i]));
+    const __half2 ha = __hmul2(*reinterpret_cast<const __half2*>(&a), scale);
+    const __half2 hb = __hmul2(*reinterpret_cast<const __half2*>(&b), scale);
+    h[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
+    h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+  }
+  lo = make_uint4(h[0], h[1], h[2], h[3]);
+  hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// S = Q K^T for one tile.
+template <int D>
+__device__ __forceinline__ void issue_qk(uint32_t d_tmem, uint64_t q_desc, uint64_t k_desc) {
+  using C = ChunkCfg<D>;
+  constexpr uint32_t IDESC = idesc_f16(false, kBM, kBN, false, false);
+  constexpr int KS = C::kKStepsPerChunk;
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k)
+    umma_ss_w(d_tmem, desc_add(q_desc, (k / KS) * C::kChunkBytes + (k % KS) * 32),
+              desc_add(k_desc, (k / KS) * C::kChunkBytes + (k % KS) * 32), IDESC, k > 0 ? 1u : 0u);
+}
+
+// O += P V over one half of the tile's keys.
+template <int D>
+__device__ __forceinline__ void issue_pv_half(uint32_t o_tmem, uint32_t p_tmem, uint64_t v_desc, uint32_t accumulate, int half) {
+  constexpr uint32_t IDESC = idesc_f16(false, kBM, D, false, true);
+  constexpr int kKeyStep = 16 * ChunkCfg<D>::kSwBytes;
+  constexpr int kSteps = kBN / 32;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int k = half * kSteps + i;
+    umma_ts_w(o_tmem, p_tmem + k * 8, desc_add(v_desc, k * kKeyStep), IDESC, (accumulate | k) ? 1u : 0u);
+  }
+}
+
+struct ChunkWork {
+  int b, h;       // sequence, K/V head; b < 0: nothing to do
+  int first, n;   // flat index of the sequence's first new token, their number
+  int before;     // keys in front of the new tokens
+  int r0;         // first of the block's 256 rows
+};
+
+// blockIdx.x -> work: sequences in order, inside a sequence the last (longest) rows first, heads
+// next to each other.  Every thread calls it.
+__device__ __forceinline__ ChunkWork find_work(const PagedParams& p, int* words) {
+  __shared__ long long warp_sum[kThreads / 32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int chunk = (p.B + kThreads - 1) / kThreads;
+  const int b0 = min(p.B, static_cast<int>(threadIdx.x) * chunk), b1 = min(p.B, b0 + chunk);
+  if (threadIdx.x == 0) words[0] = -1;
+  long long mine = 0;
+  int first = 0, n = 0, len = 0;
+  auto shape = [&](int b) {
+    first = p.offsets == nullptr ? b : p.offsets[b];
+    n = p.offsets == nullptr ? 1 : p.offsets[b + 1] - first;
+    if (first < 0 || n < 0 || first > p.T - n) {  // not inside q: no rows
+      if (n != 0) record_error(p.status, kDevBadIndex, b);
+      first = n = 0;
+    }
+    len = p.seq_lens[b];
+    if (len < 0 || len > p.capacity) {
+      record_error(p.status, kDevBadIndex, b);
+      len = 0;
+    }
+    return static_cast<long long>((n * p.group + 2 * kBM - 1) / (2 * kBM)) * p.H_kv;
+  };
+  for (int b = b0; b < b1; ++b) mine += shape(b);
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  long long before = incl - mine;
+  for (int w = 0; w < warp; ++w) before += warp_sum[w];
+  const long long item = blockIdx.x;
+  if (item >= before && item < before + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const long long items = shape(b);
+      if (item < before + items) {
+        const int i = static_cast<int>(item - before);
+        words[0] = b;
+        words[1] = i % p.H_kv;
+        words[2] = first;
+        words[3] = n;
+        words[4] = len - n;
+        words[5] = (static_cast<int>(items / p.H_kv) - 1 - i / p.H_kv) * 2 * kBM;
+        break;
+      }
+      before += items;
+    }
+  }
+  __syncthreads();
+  return {words[0], words[1], words[2], words[3], words[4], words[5]};
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedParams p) {
+  using C = ChunkCfg<D>;
+  constexpr int ST = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_base);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBar + 8 * BAR_COUNT);
+  int* words = reinterpret_cast<int*>(smem + C::kOffBar + 8 * BAR_COUNT + 16);
+  float* maxima = reinterpret_cast<float*>(smem + C::kOffBar + 8 * BAR_COUNT + 48);  // [2][16]
+  const uint32_t bar0 = smem_u32(bars);
+#define BAR(i) (bar0 + 8u * static_cast<uint32_t>(i))
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (__syncthreads_or(ld_status(p.status)) != 0) return;
+  const ChunkWork w = find_work(p, words);
+  if (w.b < 0) return;
+  const int rows = min(2 * kBM, w.n * p.group - w.r0);
+  const int ntiles = rows > kBM ? 2 : 1;
+  // keys that a tile's last row sees; a tile that sees none still runs over key 0 when the block has one
+  auto keys_of = [&](int t) {
+    const int last = w.r0 + min(rows, (t + 1) * kBM) - 1;
+    return w.before + last / p.group + 1;
+  };
+  const int keys = max(0, keys_of(ntiles - 1));  // <= the sequence's length
+  const int* table = p.block_table + w.b * p.table_stride;
+
+  if (keys == 0) {  // no row sees a key
+    for (int i = threadIdx.x; i < rows * (D / 8); i += kThreads) {
+      const int r = w.r0 + i / (D / 8), head = w.h * p.group + r % p.group;
+      const long long token = w.first + r / p.group;
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + token * p.out_stride[0] + head * p.out_stride[1] + i % (D / 8) * 8) =
+          make_uint4(0, 0, 0, 0);
+      if (p.lse != nullptr && i % (D / 8) == 0) p.lse[token * p.group * p.H_kv + head] = -INFINITY;
+    }
+    return;
+  }
+
+  // The largest page scales of the keys that the block reads.
+  float top_k = 0.f, top_v = 0.f;
+  const int pages = ((keys - 1) >> p.page_shift) + 1;
+  for (int i = threadIdx.x; i < pages; i += kThreads) {
+    const int page = table[i];
+    if (page < 0 || page >= p.num_pages) {
+      record_error(p.status, kDevBadIndex, w.b);
+    } else {
+      const size_t at = static_cast<size_t>(page) * p.H_kv + w.h;
+      const float k = p.k_scales[at], v = p.v_scales[at];
+      if (k < INFINITY) top_k = fmaxf(top_k, k);
+      if (v < INFINITY) top_v = fmaxf(top_v, v);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top_k = fmaxf(top_k, __shfl_xor_sync(0xffffffffu, top_k, o));
+    top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
+  }
+  if (lane == 0) {
+    maxima[warp] = top_k;
+    maxima[16 + warp] = top_v;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(BAR(BAR_Q), 128);
+    mbar_init(BAR(BAR_Q + 1), 128);
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(BAR(BAR_KFULL + s), 128);
+      mbar_init(BAR(BAR_KEMPTY + s), 1);
+      mbar_init(BAR(BAR_VFULL + s), 128);
+      mbar_init(BAR(BAR_VEMPTY + s), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(BAR(BAR_SFULL + t), 1);
+      mbar_init(BAR(BAR_PFULLA + t), 128);
+      mbar_init(BAR(BAR_PFULLB + t), 128);
+      mbar_init(BAR(BAR_OFULL + t), 1);
+    }
+    mbar_init(BAR(BAR_DRAIN), 1);
+    mbar_init(BAR(BAR_NEVER), 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int nkv0 = (max(1, keys_of(0)) + kBN - 1) / kBN;
+  const int nkv1 = ntiles == 2 ? (max(1, keys_of(1)) + kBN - 1) / kBN : 0;
+  const int nmax = max(nkv0, nkv1);
+  const uint32_t sK = base + C::kOffK, sV = base + C::kOffV;
+
+  if (warp >= kSoftmaxWarps) {
+    regs_decrease<kRegsOther>();
+    if (warp == kWarpMma) {
+      // ---------------------------------------------------------- UMMA issuer
+      const uint64_t dq0 = sdesc_sw(base + C::kOffQ, 16, C::kSbo, C::kLayout);
+      const uint64_t dq1 = sdesc_sw(base + C::kOffQ + C::kTileBytes, 16, C::kSbo, C::kLayout);
+      const uint64_t dk0 = sdesc_sw(sK, 16, C::kSbo, C::kLayout);
+      const uint64_t dv0 = sdesc_sw(sV, C::kChunkBytes, C::kSbo, C::kLayout);
+      const uint32_t tS0 = tmem, tS1 = tmem + 128, tO0 = tmem + 256, tO1 = tmem + 384;
+      bool ok = warp_all(mbar_wait(BAR(BAR_Q), 0, p.status, kDevTimeoutQ)) &&
+                warp_all(mbar_wait(BAR(BAR_KFULL + 0), 0, p.status, kDevTimeoutKV));
+      if (ok && nkv1 > 0) ok = warp_all(mbar_wait(BAR(BAR_Q + 1), 0, p.status, kDevTimeoutQ));
+      if (ok) {
+        tc_fence_after();
+        issue_qk<D>(tS0, dq0, dk0);
+        umma_commit_w(BAR(BAR_SFULL + 0));
+        if (nkv1 > 0) {
+          issue_qk<D>(tS1, dq1, dk0);
+          umma_commit_w(BAR(BAR_SFULL + 1));
+        }
+        umma_commit_w(BAR(BAR_KEMPTY + 0));
+      }
+      for (int j = 0; ok && j < nmax; ++j) {
+        const int vs = j % ST, ks1 = (j + 1) % ST;
+        const uint64_t dvj = dv0 + static_cast<uint64_t>((vs * C::kTileBytes) >> 4);
+        const uint64_t dkn = dk0 + static_cast<uint64_t>((ks1 * C::kTileBytes) >> 4);
+        FA_STALL_HERE(j, BAR(BAR_NEVER), p.status, ok)
+        if (!(ok = warp_all(mbar_wait(BAR(BAR_VFULL + vs), (j / ST) & 1, p.status, kDevTimeoutKV)))) break;
+        bool k_ready = false, issued_s = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int nt = t == 0 ? nkv0 : nkv1;
+          const uint32_t tS = t == 0 ? tS0 : tS1, tO = t == 0 ? tO0 : tO1;
+          if (j < nt) {
+            if (!(ok = warp_all(mbar_wait(BAR(BAR_PFULLA + t), j & 1, p.status, kDevTimeoutP)))) break;
+            tc_fence_after();
+            issue_pv_half<D>(tO, tS, dvj, j > 0 ? 1u : 0u, 0);
+            if (!(ok = warp_all(mbar_wait(BAR(BAR_PFULLB + t), j & 1, p.status, kDevTimeoutP)))) break;
+            tc_fence_after();
+            issue_pv_half<D>(tO, tS, dvj, 1u, 1);
+            if (j + 1 == nt) {
+              umma_commit_w(BAR(BAR_OFULL + t));
+            } else {
+              if (!k_ready) {
+                if (!(ok = warp_all(mbar_wait(BAR(BAR_KFULL + ks1), ((j + 1) / ST) & 1, p.status, kDevTimeoutKV)))) break;
+                tc_fence_after();
+                k_ready = true;
+              }
+              issue_qk<D>(tS, t == 0 ? dq0 : dq1, dkn);
+              umma_commit_w(BAR(BAR_SFULL + t));
+              issued_s = true;
+            }
+          }
+        }
+        if (!ok) break;
+        if (issued_s) umma_commit_w(BAR(BAR_KEMPTY + ks1));
+        umma_commit_w(BAR(BAR_VEMPTY + vs));
+      }
+      umma_commit_w(BAR(BAR_DRAIN));
+      drain_wait(BAR(BAR_DRAIN), 0, p.status);
+      __syncwarp();
+    } else if (warp >= kWarpTiles) {
+      // ---------------------------------------------------------- K and V tiles
+      constexpr int kLanes = D / 16;          // lanes of a cached row
+      constexpr int kRowsPerLoad = 32 / kLanes;
+      constexpr int kLoads = 32 / kRowsPerLoad;  // a warp's 32 rows of a tile; half of them per 16-key block
+      const int wr = (warp - kWarpTiles) * 32 + lane / kLanes;  // first row of the thread
+      const int piece = lane % kLanes;
+      const uint32_t page_bytes = static_cast<uint32_t>(D) << p.page_shift;
+      const int page_mask = (1 << p.page_shift) - 1;
+      const int last_index = pages - 1;
+      top_k = top_v = 0.f;
+      for (int i = 0; i < kThreads / 32; ++i) {
+        top_k = fmaxf(top_k, maxima[i]);
+        top_v = fmaxf(top_v, maxima[16 + i]);
+      }
+      const float inv_k = top_k > 0.f ? kHeadroom / top_k : 0.f, inv_v = top_v > 0.f ? kHeadroom / top_v : 0.f;
+      uint4 piece_raw[kLoads];
+      uint32_t factor[2];
+      auto load = [&](int j, const uint8_t* pages_ptr, const float* scales, float inv) {
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+          const int block_key = j * kBN + (warp - kWarpTiles) * 32 + 16 * blk;
+          const int page = table[min(block_key >> p.page_shift, last_index)];
+          const size_t at = static_cast<size_t>(page < 0 || page >= p.num_pages ? 0 : page) * p.H_kv + w.h;
+          const float s = scales[at] * inv;
+          const __half2 f = __float2half2_rn(s);
+          factor[blk] = *reinterpret_cast<const uint32_t*>(&f);
+          const uint8_t* src = pages_ptr + at * page_bytes + static_cast<uint32_t>(piece * 16);
+#pragma unroll
+          for (int i = 0; i < kLoads / 2; ++i) {
+            const int row = wr + (blk * (kLoads / 2) + i) * kRowsPerLoad;
+            const int key = j * kBN + row;
+            piece_raw[blk * (kLoads / 2) + i] = make_uint4(0, 0, 0, 0);  // behind the last key: zeros
+            if (key < keys)
+              piece_raw[blk * (kLoads / 2) + i] = __ldg(reinterpret_cast<const uint4*>(src + (key & page_mask) * D));
+          }
+        }
+      };
+      auto store = [&](uint8_t* tile) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int row = wr + i * kRowsPerLoad;
+          uint4 lo, hi;
+          dequant16(piece_raw[i], factor[i / (kLoads / 2)], lo, hi);
+          // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes of
+          // a row then meet all banks
+          const bool swap = D == 128 && piece >= 4;
+          *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 1 : 0))) = swap ? hi : lo;
+          *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 0 : 1))) = swap ? lo : hi;
+        }
+        fence_async_shared();
+      };
+      load(0, p.k_pages, p.k_scales, inv_k);
+      for (int j = 0; j < nmax; ++j) {
+        const int s = j % ST;
+        const uint32_t parity = ((j / ST) & 1) ^ 1;
+        if (!mbar_wait(BAR(BAR_KEMPTY + s), parity, p.status, kDevTimeoutKVEmpty)) break;
+        store(smem + C::kOffK + s * C::kTileBytes);
+        mbar_arrive(BAR(BAR_KFULL + s));
+        load(j, p.v_pages, p.v_scales, inv_v);
+        if (!mbar_wait(BAR(BAR_VEMPTY + s), parity, p.status, kDevTimeoutKVEmpty)) break;
+        store(smem + C::kOffV + s * C::kTileBytes);
+        mbar_arrive(BAR(BAR_VFULL + s));
+        if (j + 1 < nmax) load(j + 1, p.k_pages, p.k_scales, inv_k);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ softmax / epilogue, one thread per row
+    regs_increase<kRegsSoftmax>();
+    const int t = warp / 4;
+    if (t < ntiles) {
+      constexpr int NCH = kBN / 32;
+      const int wq = warp % 4;
+      const int row = wq * 32 + lane;
+      const int r = w.r0 + t * kBM + row;
+      const bool live = r < w.n * p.group;
+      const int head = w.h * p.group + r % p.group;
+      const long long token = w.first + r / p.group;
+      // the row's last key; rows that see none run over key 0 and are written as such at the end
+      const int own_last = live ? w.before + r / p.group : 0;
+      const int last = max(0, own_last);
+      const int full = max(0, w.before + (w.r0 + t * kBM) / p.group);  // every row of the tile sees keys <= full
+      top_k = top_v = 0.f;
+      for (int i = 0; i < kThreads / 32; ++i) {
+        top_k = fmaxf(top_k, maxima[i]);
+        top_v = fmaxf(top_v, maxima[16 + i]);
+      }
+      // Q row -> f16 by a power of two
+      float scale;
+      {
+        uint8_t* tile = smem + C::kOffQ + t * C::kTileBytes;
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + token * p.q_stride[0] + head * p.q_stride[1];
+        uint32_t x[D / 8][4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 v = live ? *reinterpret_cast<const uint4*>(q + 8 * c) : make_uint4(0, 0, 0, 0);
+          x[c][0] = v.x;
+          x[c][1] = v.y;
+          x[c][2] = v.z;
+          x[c][3] = v.w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max(x[c][i] & 0x7fffu, (x[c][i] >> 16) & 0x7fffu));
+        }
+        float down = 1.f;
+        if (p.bf16) {
+          const int e = min(254, max(8, static_cast<int>(top >> 7)));   // biased exponent
+          down = __uint_as_float(static_cast<uint32_t>(261 - e) << 23); // largest element to [2^7, 2^8)
+        }
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 v = make_uint4(x[c][0], x[c][1], x[c][2], x[c][3]);
+          if (p.bf16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              x[c][i] = pack2<false>(__uint_as_float(x[c][i] << 16) * down, __uint_as_float(x[c][i] & 0xffff0000u) * down);
+            v = make_uint4(x[c][0], x[c][1], x[c][2], x[c][3]);
+          }
+          *reinterpret_cast<uint4*>(tile + C::place(row, c)) = v;
+        }
+        scale = p.scale_log2 * (top_k / kHeadroom) / down;
+        fence_async_shared();
+        mbar_arrive(BAR(BAR_Q + t));
+      }
+      const int nkv = t == 0 ? nkv0 : nkv1;
+      const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+      const uint32_t tS = tmem + t * 128 + lane_off;
+      const uint32_t tO = tmem + 256 + t * 128 + lane_off;
+      float m_used = -INFINITY;
+      float l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < nkv; ++j) {
+        if (!(ok = warp_all(mbar_wait<kSoftmaxCopy>(BAR(BAR_SFULL + t), j & 1, p.status, kDevTimeoutS)))) break;
+        tc_fence_after();
+        uint32_t s[NCH][32];
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) tmem_ld32(tS + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) tmem_ld_wait(s[c]);
+        const int kbase = j * kBN;
+        const bool masked = kbase + kBN - 1 > full;
+        const uint64_t scale2 = f2(scale, scale);
+        uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+        float alpha = 1.f;
+        if (masked || j == 0) {
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (kbase + c * 32 + i > last) s[c][i] = __float_as_uint(-INFINITY);
+          }
+          const float mt = row_max<NCH>(s) * scale;
+          const bool upd = mt > m_used + kRescaleThreshold;
+          const float m_new = upd ? mt : m_used;
+          alpha = ex2_approx(m_used - m_new);
+          const uint64_t negm2 = f2(-m_new, -m_new);
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            uint32_t pk[16];
+            softmax_chunk<false, 0>(s[c], scale2, negm2, sum2, pk);
+            tmem_st16(tS + c * 16, pk);
+          }
+          if (j > 0 && __any_sync(0xffffffffu, upd)) rescale_o<D>(tO, alpha);
+          m_used = m_new;
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(BAR(BAR_PFULLA + t));
+          mbar_arrive(BAR(BAR_PFULLB + t));
+        } else {
+          // the first half with the running reference while the row's new maximum is computed beside it
+          uint64_t negm2 = f2(-m_used, -m_used);
+#pragma unroll
+          for (int c = 0; c < NCH / 2; ++c) {
+            uint32_t pk[16];
+            softmax_chunk<false, kPolyPairs>(s[c], scale2, negm2, sum2, pk);
+            tmem_st16(tS + c * 16, pk);
+          }
+          const float mt = row_max<NCH>(s) * scale;
+          const bool upd = mt > m_used + kRescaleThreshold;
+          if (__any_sync(0xffffffffu, upd)) {
+            const float m_new = upd ? mt : m_used;
+            alpha = ex2_approx(m_used - m_new);
+            negm2 = f2(-m_new, -m_new);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum2[u] = 0ull;
+#pragma unroll
+            for (int c = 0; c < NCH / 2; ++c) {
+              uint32_t pk[16];
+              softmax_chunk<false, 0>(s[c], scale2, negm2, sum2, pk);
+              tmem_st16(tS + c * 16, pk);
+            }
+            rescale_o<D>(tO, alpha);
+            m_used = m_new;
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(BAR(BAR_PFULLA + t));
+#pragma unroll
+          for (int c = NCH / 2; c < NCH; ++c) {
+            uint32_t pk[16];
+            softmax_chunk<false, kPolyPairs>(s[c], scale2, negm2, sum2, pk);
+            tmem_st16(tS + c * 16, pk);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(BAR(BAR_PFULLB + t));
+        }
+        const uint64_t s01 = fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3]));
+        l = l * alpha + (f2lo(s01) + f2hi(s01));
+      }
+      if (ok) ok = mbar_wait<kSoftmaxCopy>(BAR(BAR_OFULL + t), 0, p.status, kDevTimeoutO);
+      ok = warp_all(ok);
+      if (ok) {
+        tc_fence_after();
+        const bool seen = own_last >= 0;
+        const float f = seen ? (top_v / kHeadroom) / l : 0.f;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + token * p.out_stride[0] + head * p.out_stride[1];
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_ld_wait(o);
+          if (live) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float a = seen ? __uint_as_float(o[8 * v + 2 * i]) * f : 0.f;
+                const float b = seen ? __uint_as_float(o[8 * v + 2 * i + 1]) * f : 0.f;
+                pk[i] = p.bf16 ? pack2<true>(a, b) : pack2<false>(a, b);
+              }
+              *reinterpret_cast<uint4*>(out + c * 32 + 8 * v) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          }
+        }
+        if (p.lse != nullptr && live) p.lse[token * p.group * p.H_kv + head] = seen ? m_used + log2f(l) : -INFINITY;
+      }
+    }
+  }
+#undef BAR
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <int D>
+cudaError_t launch_chunk_t(const PagedParams& p, int blocks, cudaStream_t stream) {
+  static std::atomic<bool> smem_set[64];
+  const cudaError_t e = opt_in_smem(paged_chunk_kernel<D>, ChunkCfg<D>::kSmemBytes, smem_set, kLaunchRegs);
+  if (e != cudaSuccess) return e;
+  paged_chunk_kernel<D><<<blocks, kThreads, ChunkCfg<D>::kSmemBytes, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+// Blocks of 256 rows, at most: per K/V head, the whole ones and a last one for each sequence.
+static long long chunk_blocks(const PagedParams& p) {
+  return (static_cast<long long>(p.T) * p.group / (2 * kBM) + p.B) * p.H_kv;
+}
+
+bool use_chunk(const PagedParams& p) {
+#ifdef FA_CHUNK_ROWS
+  return static_cast<long long>(p.T) * p.group >= static_cast<long long>(FA_CHUNK_ROWS) * p.B && chunk_blocks(p) <= 0x7fffffffLL;
+#endif
+  return static_cast<long long>(p.T) * p.group >= 64LL * p.B && chunk_blocks(p) <= 0x7fffffffLL;
+}
+
+cudaError_t launch_chunk(const PagedParams& p, int D, cudaStream_t stream) {
+  const int blocks = static_cast<int>(chunk_blocks(p));
+  if (D == 32) return launch_chunk_t<32>(p, blocks, stream);
+  if (D == 64) return launch_chunk_t<64>(p, blocks, stream);
+  if (D == 128) return launch_chunk_t<128>(p, blocks, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace fa

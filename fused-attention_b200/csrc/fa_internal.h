@@ -206,6 +206,8 @@ cudaError_t launch_append(AppendParams p, int D, bool bf16, bool interleaved, cu
 int paged_row_tile(const PagedParams& p);
 int paged_blocks(const PagedParams& p, int D);  // size of the split kernel's grid
 cudaError_t launch_paged(const PagedParams& p, int D, int blocks, cudaStream_t stream);
+bool use_chunk(const PagedParams& p);  // whether the chunk kernel takes the call
+cudaError_t launch_chunk(const PagedParams& p, int D, cudaStream_t stream);
 
 // Launchers implemented in the kernel translation units.  They return a cudaError_t.
 cudaError_t launch_fwd(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,

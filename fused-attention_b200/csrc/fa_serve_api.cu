@@ -225,6 +225,10 @@ int fa_paged_attention(const fa_paged_args* a, int* dev_status, void* stream) {
   p.capacity = a->width * a->page_size;
   p.bf16 = a->dtype == FA_DTYPE_BF16;
   p.scale_log2 = a->scale * 1.4426950408889634f;
+  if (fa::use_chunk(p)) {
+    const cudaError_t e = fa::launch_chunk(p, a->D, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FA_OK : fa::cuda_fail(e);
+  }
   const int blocks = fa::paged_blocks(p, a->D);
   const size_t rows = 2 * static_cast<size_t>(blocks) * fa::paged_row_tile(p);
   p.joins = static_cast<fa::PagedJoin*>(a->workspace);  // 24 bytes each, then 16-byte aligned arrays
