@@ -13,14 +13,14 @@
 //     relative to the sequence's largest, ref: f16(64 v8 scale / ref) is exact for power-of-two scales
 //     down to 2^-21 of the largest (below, values keep an absolute precision of 2^-40 of the largest page's
 //     magnitude; scales that are no powers of two are rounded to f16's 11 bits).  So S and O need no
-//     per-page arithmetic, and the 64 keys-by-key conversions cost the softmax warps nothing;
+//     per-page arithmetic, and the conversions cost the softmax warps nothing;
 //   * queries are brought to f16 by a power of two per row (exact down to 2^-31 of the row's largest
 //     element) by the thread that owns the row; P is f16.
 // Warp roles (512 threads):
 //   warps 0-3, 4-7  softmax warpgroups of query tiles 0 and 1 (they load Q and write O)
 //   warp 8          UMMA issuer: S_t = Q_t K_j^T, O_t += P_t V_j with P_t in TMEM
-//   warps 9-11      idle
-//   warps 12-15     K and V tiles
+//   warps 9-11      V tiles: 16-key blocks, three, three and two of a tile's eight
+//   warps 12-15     K tiles: two 16-key blocks each
 // Registers: 128 a thread at launch; warps 8-15 drop to kRegsOther, the softmax warps rise to
 // kRegsSoftmax, and 256 x kRegsOther + 256 x kRegsSoftmax = 512 x 128.
 // TMEM (512 columns): S_0 | S_1 | O_0 | O_1, P_t over the first half of S_t; P is published in two halves.
@@ -36,7 +36,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kWarpMma = 8;
-constexpr int kWarpTiles = 12;  // first of the four warps that build K and V tiles
+constexpr int kWarpV = 9;        // first of the three warps that build V tiles
+constexpr int kWarpK = 12;       // first of the four warps that build K tiles
 constexpr int kBM = 128;
 constexpr int kBN = 128;
 constexpr uint32_t kTmemCols = 512;
@@ -61,7 +62,8 @@ struct ChunkCfg {
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = 2 * kTileBytes;
   static constexpr int kOffV = kOffK + kStages * kTileBytes;
-  static constexpr int kOffBar = kOffV + kStages * kTileBytes;
+  static constexpr int kOffRaw = kOffV + kStages * kTileBytes;  // the next K and V tiles' cached bytes
+  static constexpr int kOffBar = kOffRaw + 2 * 128 * D;
   static constexpr int kSmemBytes = kOffBar + 512 + 1024;  // barriers, scan words, alignment slack
   // Byte offset of 16-byte piece c of row r of an f16 tile (pieces of D / 8 per row).
   static __device__ __forceinline__ uint32_t place(int r, int c) {
@@ -261,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
     for (int s = 0; s < 4; ++s) {
       mbar_init(BAR(BAR_KFULL + s), 128);
       mbar_init(BAR(BAR_KEMPTY + s), 1);
-      mbar_init(BAR(BAR_VFULL + s), 128);
+      mbar_init(BAR(BAR_VFULL + s), 96);
       mbar_init(BAR(BAR_VEMPTY + s), 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -348,71 +350,89 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       umma_commit_w(BAR(BAR_DRAIN));
       drain_wait(BAR(BAR_DRAIN), 0, p.status);
       __syncwarp();
-    } else if (warp >= kWarpTiles) {
-      // ---------------------------------------------------------- K and V tiles
-      constexpr int kLanes = D / 16;          // lanes of a cached row
+    } else {
+      // ---------------------------------------------------------- K and V tiles, 16 keys at a time
+      constexpr int kLanes = D / 16;             // lanes of a cached row
       constexpr int kRowsPerLoad = 32 / kLanes;
-      constexpr int kLoads = 32 / kRowsPerLoad;  // a warp's 32 rows of a tile; half of them per 16-key block
-      const int wr = (warp - kWarpTiles) * 32 + lane / kLanes;  // first row of the thread
-      const int piece = lane % kLanes;
+      constexpr int kLoads = 16 / kRowsPerLoad;  // a thread's pieces of a block
+      const bool is_k = warp >= kWarpK;
+      const int first_block = is_k ? 2 * (warp - kWarpK) : 3 * (warp - kWarpV);
+      const int blocks = is_k ? 2 : (warp == kWarpV + 2 ? 2 : 3);
+      constexpr int kMost = 3;                   // blocks of a warp, at most
+      const int row_in_block = lane / kLanes, piece = lane % kLanes;
+      const uint8_t* bytes = (is_k ? p.k_pages : p.v_pages) + piece * 16;
+      const float* scales = is_k ? p.k_scales : p.v_scales;
+      uint8_t* ring = smem + (is_k ? C::kOffK : C::kOffV);
+      // A block's bytes wait in shared memory (asynchronous copies, each thread its own pieces) from the
+      // moment the block of the tile before has been converted: nearly a tile's time in flight.
+      const uint8_t* raw = smem + C::kOffRaw + (is_k ? 0 : 128 * D) + first_block * 16 * D + lane * 16;
+      const uint32_t full = BAR(is_k ? BAR_KFULL : BAR_VFULL), empty = BAR(is_k ? BAR_KEMPTY : BAR_VEMPTY);
       const uint32_t page_bytes = static_cast<uint32_t>(D) << p.page_shift;
       const int page_mask = (1 << p.page_shift) - 1;
-      const int last_index = pages - 1;
-      top_k = top_v = 0.f;
-      for (int i = 0; i < kThreads / 32; ++i) {
-        top_k = fmaxf(top_k, maxima[i]);
-        top_v = fmaxf(top_v, maxima[16 + i]);
-      }
-      const float inv_k = top_k > 0.f ? kHeadroom / top_k : 0.f, inv_v = top_v > 0.f ? kHeadroom / top_v : 0.f;
-      uint4 piece_raw[kLoads];
-      uint32_t factor[2];
-      auto load = [&](int j, const uint8_t* pages_ptr, const float* scales, float inv) {
+      float top = 0.f;
+      for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, maxima[(is_k ? 0 : 16) + i]);
+      const float inv = top > 0.f ? kHeadroom / top : 0.f;
+      int page[kMost] = {};     // of the block's next copy, read a tile ahead
+      float scale[kMost] = {};  // of the bytes that wait
+      auto page_of = [&](int j, int blk) {
+        return table[min((j * kBN + (first_block + blk) * 16) >> p.page_shift, pages - 1)];
+      };
+      auto copy = [&](int j, int blk) {
+        if (j < nmax) {
+          const int key0 = j * kBN + (first_block + blk) * 16;
+          const size_t at = static_cast<size_t>(page[blk] < 0 || page[blk] >= p.num_pages ? 0 : page[blk]) * p.H_kv + w.h;
+          // rows behind the last key are inside the page: read, and cleared when they are converted
+          const uint8_t* src = bytes + at * page_bytes + (key0 & page_mask) * D + row_in_block * D;
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-          const int block_key = j * kBN + (warp - kWarpTiles) * 32 + 16 * blk;
-          const int page = table[min(block_key >> p.page_shift, last_index)];
-          const size_t at = static_cast<size_t>(page < 0 || page >= p.num_pages ? 0 : page) * p.H_kv + w.h;
-          const float s = scales[at] * inv;
-          const __half2 f = __float2half2_rn(s);
-          factor[blk] = *reinterpret_cast<const uint32_t*>(&f);
-          const uint8_t* src = pages_ptr + at * page_bytes + static_cast<uint32_t>(piece * 16);
+          for (int i = 0; i < kLoads; ++i)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + blk * 16 * D + i * 512)),
+                         "l"(src + i * 512) : "memory");
+          scale[blk] = scales[at];
+          page[blk] = page_of(j + 1, blk);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
 #pragma unroll
-          for (int i = 0; i < kLoads / 2; ++i) {
-            const int row = wr + (blk * (kLoads / 2) + i) * kRowsPerLoad;
-            const int key = j * kBN + row;
-            piece_raw[blk * (kLoads / 2) + i] = make_uint4(0, 0, 0, 0);  // behind the last key: zeros
-            if (key < keys)
-              piece_raw[blk * (kLoads / 2) + i] = __ldg(reinterpret_cast<const uint4*>(src + (key & page_mask) * D));
+      for (int blk = 0; blk < kMost; ++blk) page[blk] = page_of(0, blk);
+#pragma unroll
+      for (int blk = 0; blk < kMost; ++blk)
+        if (blk < blocks) copy(0, blk);
+      bool ok = true;
+      for (int j = 0; ok && j < nmax; ++j) {
+        const int st = j % ST;
+        uint8_t* tile = ring + st * C::kTileBytes;
+        if (!(ok = mbar_wait(empty + 8 * st, ((j / ST) & 1) ^ 1, p.status, kDevTimeoutKVEmpty))) break;
+#pragma unroll
+        for (int blk = 0; blk < kMost; ++blk) {
+          if (blk < blocks) {
+            // the oldest of the warp's `blocks` copies in flight has landed
+            if (blocks == 2)
+              asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else
+              asm volatile("cp.async.wait_group 2;" ::: "memory");
+            const __half2 f2h = __float2half2_rn(scale[blk] * inv);
+            const uint32_t factor = *reinterpret_cast<const uint32_t*>(&f2h);
+            const int row0 = (first_block + blk) * 16 + row_in_block;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+              const int row = row0 + i * kRowsPerLoad;
+              uint4 v = *reinterpret_cast<const uint4*>(raw + blk * 16 * D + i * 512);
+              if (j * kBN + row >= keys) v = make_uint4(0, 0, 0, 0);  // behind the last key
+              uint4 lo, hi;
+              dequant16(v, factor, lo, hi);
+              // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes
+              // of a row then meet all banks
+              const bool swap = D == 128 && piece >= 4;
+              *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 1 : 0))) = swap ? hi : lo;
+              *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 0 : 1))) = swap ? lo : hi;
+            }
+            copy(j + 1, blk);
           }
         }
-      };
-      auto store = [&](uint8_t* tile) {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int row = wr + i * kRowsPerLoad;
-          uint4 lo, hi;
-          dequant16(piece_raw[i], factor[i / (kLoads / 2)], lo, hi);
-          // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes of
-          // a row then meet all banks
-          const bool swap = D == 128 && piece >= 4;
-          *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 1 : 0))) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 0 : 1))) = swap ? lo : hi;
-        }
         fence_async_shared();
-      };
-      load(0, p.k_pages, p.k_scales, inv_k);
-      for (int j = 0; j < nmax; ++j) {
-        const int s = j % ST;
-        const uint32_t parity = ((j / ST) & 1) ^ 1;
-        if (!mbar_wait(BAR(BAR_KEMPTY + s), parity, p.status, kDevTimeoutKVEmpty)) break;
-        store(smem + C::kOffK + s * C::kTileBytes);
-        mbar_arrive(BAR(BAR_KFULL + s));
-        load(j, p.v_pages, p.v_scales, inv_v);
-        if (!mbar_wait(BAR(BAR_VEMPTY + s), parity, p.status, kDevTimeoutKVEmpty)) break;
-        store(smem + C::kOffV + s * C::kTileBytes);
-        mbar_arrive(BAR(BAR_VFULL + s));
-        if (j + 1 < nmax) load(j + 1, p.k_pages, p.k_scales, inv_k);
+        mbar_arrive(full + 8 * st);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
     }
   } else {
@@ -616,11 +636,21 @@ static long long chunk_blocks(const PagedParams& p) {
   return (static_cast<long long>(p.T) * p.group / (2 * kBM) + p.B) * p.H_kv;
 }
 
-bool use_chunk(const PagedParams& p) {
-#ifdef FA_CHUNK_ROWS
-  return static_cast<long long>(p.T) * p.group >= static_cast<long long>(FA_CHUNK_ROWS) * p.B && chunk_blocks(p) <= 0x7fffffffLL;
+// Which kernel takes a call, by the two's times for its 128-key tiles.  The split kernel spends c1 = 7 ns of
+// the whole GPU on 16 rows and 128 keys at D = 128 (4.2 ns at D = 64), the chunk kernel c2 = 2.25 us (1.6 us)
+// of one SM on 256 rows, filled or not: c2 / c1 is about 320 at D = 128 and 400 below.  Measured at D = 128,
+// 8 K/V heads, groups of 4, 8192 keys, chunk / split: 16 x 16 tokens 152 / 244 us, 1 x 256 tokens 167 / 215,
+// 4 x 16 tokens 144 / 78, 1 x 64 tokens 165 / 74.  Only averages are known here: sequences' lengths are on the device.
+bool use_chunk(const PagedParams& p, int D) {
+  if (chunk_blocks(p) > 0x7fffffffLL) return false;
+#ifdef FA_CHUNK_ROWS  // a build that picks by rows alone, to time one kernel against the other
+  return static_cast<long long>(p.T) * p.group >= static_cast<long long>(FA_CHUNK_ROWS) * p.B;
+#else
+  const long long rows = (static_cast<long long>(p.T) * p.group + p.B - 1) / p.B;  // of a sequence and K/V head
+  const long long items = static_cast<long long>(p.B) * p.H_kv;
+  const long long waves = (items * ((rows + 2 * kBM - 1) / (2 * kBM)) + 147) / 148;
+  return items * ((rows + 15) / 16) >= (D == 128 ? 320 : 400) * waves;
 #endif
-  return static_cast<long long>(p.T) * p.group >= 64LL * p.B && chunk_blocks(p) <= 0x7fffffffLL;
 }
 
 cudaError_t launch_chunk(const PagedParams& p, int D, cudaStream_t stream) {

@@ -116,11 +116,12 @@ struct AppendParams {
   long long pos_axis_stride;
   double eps;
   int* status;
-  int T, B, width, num_pages, H_kv, page_size;
+  int T, B, width, num_pages, H_kv;
+  int page_shift;            // log2(page size)
   int max_pos, axes;
   int section_start[kRopeMaxAxes];
   int pos64, weight_f32;
-  int window;                // tokens of a block, set by the launcher
+  int window, slices;        // tokens and slices of a block, set by the launcher
 };
 
 // A cut tile of rows: its opening part is in `slot`, the others in the first slots of the blocks after.
@@ -206,7 +207,7 @@ cudaError_t launch_append(AppendParams p, int D, bool bf16, bool interleaved, cu
 int paged_row_tile(const PagedParams& p);
 int paged_blocks(const PagedParams& p, int D);  // size of the split kernel's grid
 cudaError_t launch_paged(const PagedParams& p, int D, int blocks, cudaStream_t stream);
-bool use_chunk(const PagedParams& p);  // whether the chunk kernel takes the call
+bool use_chunk(const PagedParams& p, int D);  // whether the chunk kernel takes the call
 cudaError_t launch_chunk(const PagedParams& p, int D, cudaStream_t stream);
 
 // Launchers implemented in the kernel translation units.  They return a cudaError_t.

@@ -12,6 +12,8 @@ bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(
 
 bool head_dim_ok(int D) { return D == 32 || D == 64 || D == 128; }
 
+int page_shift(int page_size) { return page_size == 16 ? 4 : (page_size == 32 ? 5 : (page_size == 64 ? 6 : 7)); }
+
 // Strides of 16-bit rows: multiples of 8 elements (16 bytes).
 template <int N>
 bool strides_ok(const long long (&s)[N]) {
@@ -177,7 +179,7 @@ int fa_append_kv(const fa_append_args* a, int* dev_status, void* stream) {
   p.width = a->width;
   p.num_pages = a->num_pages;
   p.H_kv = a->H_kv;
-  p.page_size = a->page_size;
+  p.page_shift = page_shift(a->page_size);
   p.max_pos = a->max_pos;
   p.axes = a->axes;
   p.pos64 = a->pos_is_int64;
@@ -221,11 +223,11 @@ int fa_paged_attention(const fa_paged_args* a, int* dev_status, void* stream) {
   p.num_pages = a->num_pages;
   p.H_kv = a->H_kv;
   p.group = a->H / a->H_kv;
-  p.page_shift = a->page_size == 16 ? 4 : (a->page_size == 32 ? 5 : (a->page_size == 64 ? 6 : 7));
+  p.page_shift = page_shift(a->page_size);
   p.capacity = a->width * a->page_size;
   p.bf16 = a->dtype == FA_DTYPE_BF16;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  if (fa::use_chunk(p)) {
+  if (fa::use_chunk(p, a->D)) {
     const cudaError_t e = fa::launch_chunk(p, a->D, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FA_OK : fa::cuda_fail(e);
   }
