@@ -130,6 +130,7 @@ struct Cursor {
   long long total;  // units of the call
   int b;            // sequence of the share's first unit
   long long skip;   // units of that sequence before it
+  bool stop;        // the status word was set
 };
 
 __device__ __forceinline__ void sequence_shape(const PagedParams& p, int b, int& first, int& n, int& len) {
@@ -163,7 +164,7 @@ __device__ __forceinline__ long long active_blocks(long long total) {
 }
 
 template <int RT>
-__device__ __forceinline__ Cursor find_share(const PagedParams& p) {
+__device__ __forceinline__ Cursor find_share(const PagedParams& p, int status) {
   __shared__ long long warp_sum[kWarps];
   __shared__ long long found[2];
   const int chunk = (p.B + kPagedThreads - 1) / kPagedThreads;
@@ -209,7 +210,7 @@ __device__ __forceinline__ Cursor find_share(const PagedParams& p) {
       }
     }
   }
-  __syncthreads();
+  c.stop = __syncthreads_or(status) != 0;
   c.b = static_cast<int>(found[0]);
   c.skip = found[1];
   return c;
@@ -338,14 +339,11 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
   __shared__ float sh_o[kWarps][RT][D + 4];  // +4: rows start on different banks
   __shared__ float sh_m[kWarps][RT], sh_l[kWarps][RT];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (__syncthreads_or(ld_status(p.status)) != 0) {
-    if (threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
-    return;
-  }
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int g = lane / 4, t = lane % 4;
-  const Cursor cur = find_share<RT>(p);
   if (threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
+  const Cursor cur = find_share<RT>(p, ld_status(p.status));
+  if (cur.stop) return;
   const long long blocks = active_blocks(cur.total);
   if (static_cast<long long>(blockIdx.x) >= blocks) return;
   long long unit = cur.total * blockIdx.x / blocks;
