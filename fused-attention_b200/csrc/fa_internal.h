@@ -134,7 +134,7 @@ struct PagedJoin {
 };
 
 // Parameters of attention over the paged cache (fa_paged.cu).
-constexpr int kPagedUnit = 64;
+constexpr int kPagedUnit = 128;
 struct PagedParams {
   const void* q;             // [T, H, D], strides below
   const uint8_t* k_pages;
