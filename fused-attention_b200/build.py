@@ -33,7 +33,7 @@ STALL_FLAGS = ["-DFA_TEST_STALL_STEP=1", "-DFA_WAIT_TIMEOUT_NS=20000000ull"]
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 SOURCES = ["fa_api.cu", "fa_fwd.cu", "fa_bwd.cu", "fa_noalloc.cu", "fa_unfused.cu",
            "fa_rope.cu", "fa_append.cu", "fa_paged.cu", "fa_chunk.cu", "fa_serve_api.cu"]
-HEADERS = ["fa_sm100.cuh", "fa_softmax.cuh", "fa_internal.h"]
+HEADERS = ["fa_sm100.cuh", "fa_paged.cuh", "fa_softmax.cuh", "fa_internal.h"]
 
 NVCC = os.environ.get("NVCC", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

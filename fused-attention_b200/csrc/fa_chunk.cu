@@ -25,6 +25,7 @@
 // kRegsSoftmax, and 256 x kRegsOther + 256 x kRegsSoftmax = 512 x 128.
 // TMEM (512 columns): S_0 | S_1 | O_0 | O_1, P_t over the first half of S_t; P is published in two halves.
 #include "fa_internal.h"
+#include "fa_paged.cuh"
 #include "fa_sm100.cuh"
 #include "fa_softmax.cuh"
 
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (__syncthreads_or(ld_status(p.status)) != 0) return;
+  clear_unowned_rows<D>(p);
   const ChunkWork w = find_work(p, words);
   if (w.b < 0) return;
   const int rows = min(2 * kBM, w.n * p.group - w.r0);

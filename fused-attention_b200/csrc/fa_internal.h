@@ -157,6 +157,7 @@ struct PagedParams {
   int page_shift;            // log2(page size)
   int capacity;              // tokens that a row of the table can name
   int bf16;
+  int clear_unowned;         // rows of tokens that no sequence has are cleared
   float scale_log2;          // log2(e) * softmax scale
 };
 

@@ -8,8 +8,8 @@
 // Bound: HBM.  A decode step reads every cached byte once and does 4 G D operations on 2 D bytes
 // (G query heads per K/V head), so what counts is bytes in flight and few instructions per byte.
 //   * Units.  The rows of a (sequence, K/V head), n tokens x G heads, form tiles of 8 NT rows; the
-//     tile's keys form units of kUnit keys, one 32-key tile for each warp.  All units of the call, in order, are cut into equal
-//     contiguous shares, one per block of a single wave: no block has more than its share however
+//     tile's keys form units of kUnit keys, one 32-key tile for each warp.  All units
+//     of the call, in order, are cut into equal contiguous shares, one per block of a single wave: no block has more than its share however
 //     ragged the lengths are, and there is no atomic and no order that depends on timing.  A tile
 //     that is cut is written as partial results and joined by the second kernel, in a fixed order.
 //     Measured with D = 128: 128 sequences of 4096 keys and 8 K/V heads 176 us, 6.1 TB/s or 93 % of the
@@ -32,6 +32,7 @@
 //     only when a score passes it by 2^kSlack: O is rescaled, and lanes compare notes, only then.
 //   K of the next tile is loaded before the softmax of this one, V of this one before its S.
 #include "fa_internal.h"
+#include "fa_paged.cuh"
 #include "fa_sm100.cuh"
 
 #include <cuda_fp8.h>
@@ -347,6 +348,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
   if (threadIdx.x == 0) p.joins[blockIdx.x].parts = 0;
   const Cursor cur = find_share<RT>(p, ld_status(p.status));
   if (cur.stop) return;
+  clear_unowned_rows<D>(p);
   const long long blocks = active_blocks(cur.total);
   if (static_cast<long long>(blockIdx.x) >= blocks) return;
   long long unit = cur.total * blockIdx.x / blocks;

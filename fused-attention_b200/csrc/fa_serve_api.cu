@@ -226,6 +226,7 @@ int fa_paged_attention(const fa_paged_args* a, int* dev_status, void* stream) {
   p.page_shift = page_shift(a->page_size);
   p.capacity = a->width * a->page_size;
   p.bf16 = a->dtype == FA_DTYPE_BF16;
+  p.clear_unowned = a->clear_unowned;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   if (fa::use_chunk(p, a->D)) {
     const cudaError_t e = fa::launch_chunk(p, a->D, static_cast<cudaStream_t>(stream));

@@ -424,9 +424,11 @@ py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, 
   if (out_opt.has_value())
     out = *out_opt;
   else
-    out = offsets.has_value() || B == 0 ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());
-  Tensor lse;
-  if (return_lse) lse = at::full({T, H}, -std::numeric_limits<double>::infinity(), q.options().dtype(at::kFloat));
+    out = B == 0 ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());
+  Tensor lse;  // with the caller's out, rows that no sequence has are not written
+  if (return_lse)
+    lse = B == 0 || out_opt.has_value() ? at::full({T, H}, -std::numeric_limits<double>::infinity(), q.options().dtype(at::kFloat))
+                                        : at::empty({T, H}, q.options().dtype(at::kFloat));
   if (T > 0 && B > 0) {
     fa_paged_args a{};
     const Tensor qr = rows(q, a.q_stride);
@@ -453,6 +455,7 @@ py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, 
     a.page_size = static_cast<int>(kp.size(2));
     a.D = static_cast<int>(D);
     a.dtype = type_code(q);
+    a.clear_unowned = !out_opt.has_value();
     a.scale = static_cast<float>(scale);
     call(fa_paged_attention, a, q, "paged_attention");
   }

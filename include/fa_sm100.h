@@ -185,7 +185,7 @@ FA_API int fa_append_kv(const struct fa_append_args* args, int* dev_status, void
 
 /* Attention of T query tokens ([T, H, D]) over the cache: query token i of sequence b's n new tokens
  * sees its keys j <= seq_lens[b] - n + i.  out [T, H, D]; lse [T, H] (log2 domain) or NULL; a row
- * that sees no key gets 0 and -inf.  Tokens behind offsets[B] are left as they are. */
+ * that sees no key gets 0 and -inf. */
 struct fa_paged_args {
   const void* q;
   const void *k_pages, *v_pages;
@@ -197,6 +197,7 @@ struct fa_paged_args {
   long long q_stride[2], out_stride[2]; /* token, head */
   long long table_stride;
   int T, B, width, num_pages, H, H_kv, page_size, D, dtype;
+  int clear_unowned;           /* nonzero: tokens that no sequence has get 0 and -inf, else they stay as they are */
   float scale;
 };
 FA_API int fa_paged_attention(const struct fa_paged_args* args, int* dev_status, void* stream);

@@ -23,7 +23,7 @@ def _nat():
 # The structs of include/fa_sm100.h, field by field.
 NORM_ROPE_ARGS = struct.Struct("@16P14q15if")
 APPEND_ARGS = struct.Struct("@13P6qd18i")
-PAGED_ARGS = struct.Struct("@11P5q9if")
+PAGED_ARGS = struct.Struct("@11P5q10if4x")
 
 
 def half(*shape, dtype=torch.float16):
@@ -164,7 +164,7 @@ def test_packed_arguments_match_the_header(tmp_path):
     """The formats that these tests pack with have the size and offsets that a C compiler gives the header's structs."""
     fields = {"fa_norm_rope_args": (NORM_ROPE_ARGS, ["q_stride", "B", "eps"], [16 * 8, 16 * 8 + 14 * 8, 16 * 8 + 14 * 8 + 15 * 4]),
               "fa_append_args": (APPEND_ARGS, ["k_stride", "eps", "T"], [13 * 8, 19 * 8, 20 * 8]),
-              "fa_paged_args": (PAGED_ARGS, ["q_stride", "T", "scale"], [11 * 8, 16 * 8, 16 * 8 + 9 * 4])}
+              "fa_paged_args": (PAGED_ARGS, ["q_stride", "T", "scale"], [11 * 8, 16 * 8, 16 * 8 + 10 * 4])}
     src = "#include <stdio.h>\n#include <stddef.h>\n#include \"fa_sm100.h\"\nint main(void) {\n"
     for name, (_, members, _) in fields.items():
         src += f'printf("%zu", sizeof(struct {name}));\n'
@@ -192,7 +192,7 @@ AP = dict(k=256, v=256, kp=256, vp=256, ks=256, vs=256, table=256, lens=256, off
           st=[64] * 6, eps=1e-6, T=3, B=3, width=2, pages=4, H_kv=2, P=16, D=64, dtype=0, wdtype=0, max_pos=0, axes=1,
           s0=0, s1=0, s2=0, s3=0, pos64=0, inter=0, reserved=0)
 PA = dict(q=256, kp=256, vp=256, ks=256, vs=256, table=256, lens=256, offsets=0, out=256, lse=0, ws=256, st=[64] * 5,
-          T=3, B=3, width=2, pages=4, H=4, H_kv=2, P=16, D=64, dtype=0, scale=0.125)
+          T=3, B=3, width=2, pages=4, H=4, H_kv=2, P=16, D=64, dtype=0, clear=0, scale=0.125)
 
 
 def _packed(packer, base, **kw):
