@@ -29,7 +29,7 @@
 #include "fa_sm100.cuh"
 #include "fa_softmax.cuh"
 
-#include <cuda_fp8.h>
+#include <type_traits>
 
 namespace fa {
 namespace {
@@ -88,7 +88,10 @@ enum : int {
   BAR_COUNT = 28
 };
 
-// One 16-byte piece of a cached row -> 16 f16 values times f.
+// One 16-byte piece of a cached row -> 16 f16 values times f, or times f 2^-14 where `small`: the first product is
+// exact (a byte's value is a multiple of 2^-9), so there is one rounding either way.
+constexpr float kSmall = 1.f / 16384;  // f16's smallest normal number: a smaller factor would lose bits itself
+template <bool small>
 __device__ __forceinline__ void dequant16(const uint4& raw, uint32_t f, uint4& lo, uint4& hi) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   uint32_t h[8];
@@ -98,8 +101,13 @@ __device__ __forceinline__ void dequant16(const uint4& raw, uint32_t f, uint4& l
     uint32_t a, b;
     asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
         : "=r"(a), "=r"(b) : "r"(w[i]));
-    const __half2 ha = __hmul2(*reinterpret_cast<const __half2*>(&a), scale);
-    const __half2 hb = __hmul2(*reinterpret_cast<const __half2*>(&b), scale);
+    __half2 ha = *reinterpret_cast<const __half2*>(&a), hb = *reinterpret_cast<const __half2*>(&b);
+    if constexpr (small) {
+      ha = __hmul2(ha, __float2half2_rn(kSmall));
+      hb = __hmul2(hb, __float2half2_rn(kSmall));
+    }
+    ha = __hmul2(ha, scale);
+    hb = __hmul2(hb, scale);
     h[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
     h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
   }
@@ -412,22 +420,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
               asm volatile("cp.async.wait_group 1;" ::: "memory");
             else
               asm volatile("cp.async.wait_group 2;" ::: "memory");
-            const __half2 f2h = __float2half2_rn(scale[blk] * inv);
+            const float relative = scale[blk] * inv;
+            const bool small = relative < kSmall;
+            const __half2 f2h = __float2half2_rn(small ? relative * (1.f / kSmall) : relative);
             const uint32_t factor = *reinterpret_cast<const uint32_t*>(&f2h);
             const int row0 = (first_block + blk) * 16 + row_in_block;
+            auto convert = [&](auto is_small) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-              const int row = row0 + i * kRowsPerLoad;
-              uint4 v = *reinterpret_cast<const uint4*>(raw + blk * 16 * D + i * 512);
-              if (j * kBN + row >= keys) v = make_uint4(0, 0, 0, 0);  // behind the last key
-              uint4 lo, hi;
-              dequant16(v, factor, lo, hi);
-              // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes
-              // of a row then meet all banks
-              const bool swap = D == 128 && piece >= 4;
-              *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 1 : 0))) = swap ? hi : lo;
-              *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 0 : 1))) = swap ? lo : hi;
-            }
+              for (int i = 0; i < kLoads; ++i) {
+                const int row = row0 + i * kRowsPerLoad;
+                uint4 v = *reinterpret_cast<const uint4*>(raw + blk * 16 * D + i * 512);
+                if (j * kBN + row >= keys) v = make_uint4(0, 0, 0, 0);  // behind the last key
+                uint4 lo, hi;
+                dequant16<decltype(is_small)::value>(v, factor, lo, hi);
+                // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes
+                // of a row then meet all banks
+                const bool swap = D == 128 && piece >= 4;
+                *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 1 : 0))) = swap ? hi : lo;
+                *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 0 : 1))) = swap ? lo : hi;
+              }
+            };
+            if (small)
+              convert(std::true_type{});
+            else
+              convert(std::false_type{});
             copy(j + 1, blk);
           }
         }

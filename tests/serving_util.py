@@ -107,7 +107,7 @@ def append64(kp, vp, ks, vs, k, v, table, lens, starts, c, s, w, eps, interleave
     return kp, vp, ks, vs
 
 
-def paged64(q, kp, vp, ks, vs, table, lens, starts, scale):
+def paged64(q, kp, vp, ks, vs, table, lens, starts, scale, chunk=False):
     """(o, lse, bound, lse_bound) of paged attention in 64 bits; `bound` is what the kernels' arithmetic may add to
     half a step of the output's type, `lse_bound` how far lse may be off (all CPU tensors):
       * a score is a float32 sum of D exact products: off by at most 2 D 2^-24 of the sum of their magnitudes
@@ -115,7 +115,11 @@ def paged64(q, kp, vp, ks, vs, table, lens, starts, scale):
         the same again, plus 2^-20 for the exponentials, holds for the softmax sum;
       * a weight is rounded to f16: 2^-11 of it, or 2^-25 of the largest weight times page scale;
       * the weighted sum over n keys is a float32 sum: 2 n 2^-24 of the sum of magnitudes;
-      * lse: the scores' error, the softmax sum's (2^-20 and n 2^-24, relative) and two float32 roundings."""
+      * lse: the scores' error, the softmax sum's (2^-20 and n 2^-24, relative) and two float32 roundings.
+    The chunk kernel (chunk=True) adds:
+      * a share of the exponentials as a polynomial, 7.5e-5 < 2^-13 of them, in the weights and in their sum;
+      * weights relative to the largest weight alone: 2^-25 of it times the sum of |v|;
+      * cached values as f16(64 value / largest page scale): 2^-25 of 1/64 of that scale, where f16 is subnormal."""
     T, H, D = q.shape
     P, H_kv = kp.shape[2], kp.shape[1]
     G = H // H_kv
@@ -127,26 +131,33 @@ def paged64(q, kp, vp, ks, vs, table, lens, starts, scale):
     for b, L in enumerate(lens):
         n = starts[b + 1] - starts[b]
         pages = [int(table[b, i]) for i in range(-(-L // P))]
-        if not pages or n == 0:
+        skip = max(0, n - L)  # tokens in front of the first key
+        if not pages or n <= skip:
             continue
+        t = slice(starts[b] + skip, starts[b + 1])
         K = (kp[pages].double() * ks[pages].double()[..., None, None]).transpose(1, 2).reshape(-1, H_kv, D)[:L]
         code = vp[pages].double().transpose(1, 2).reshape(-1, H_kv, D)[:L]
         size = vs[pages].double()[:, None].expand(-1, P, -1).reshape(-1, H_kv)[:L]
-        for i in range(n):
-            m = L - n + i + 1
-            if m <= 0:
-                continue
-            for h in range(H):
-                g = h // G
-                x = (K[:m, g] @ q[starts[b] + i, h]) * scale
-                off = float(((K[:m, g].abs() @ q[starts[b] + i, h].abs()) * scale).max()) * 2 * D * U32
-                p = torch.softmax(x, 0)
-                V = code[:m, g] * size[:m, g, None]
-                t = starts[b] + i
-                o[t, h] = p @ V
-                lse[t, h] = torch.logsumexp(x, 0) * math.log2(math.e)
-                lse_bound[t, h] = math.log2(math.e) * (off + 2.0 ** -20 + m * U32) + 4 * U32 * (1 + abs(float(lse[t, h])))
-                most = float((p * size[:m, g]).max())
-                bound[t, h] = (p @ V.abs()) * (2.0 ** -11 + 2 * off + 2.0 ** -19 + 4 * m * U32) \
-                    + 2.0 ** -25 * most * code[:m, g].abs().sum(0)
+        count = torch.arange(L - n + skip, L)[:, None] + 1.0  # keys that each token sees
+        hidden = torch.arange(L)[None] >= count
+        for h in range(H):
+            g = h // G
+            k, v, row = K[:, g], code[:, g] * size[:, g, None], q[t, h]
+            x = (row @ k.T * scale).masked_fill(hidden, -math.inf)
+            off = (row.abs() @ k.abs().T * scale).masked_fill(hidden, 0).amax(1, keepdim=True) * 2 * D * U32
+            p = torch.softmax(x, 1)
+            o[t, h] = p @ v
+            lse[t, h] = torch.logsumexp(x, 1) * math.log2(math.e)
+            weight = 2.0 ** -11 + 2.0 ** -19 + 4 * count * U32
+            more = 0.0
+            if chunk:
+                off = off + row.abs().sum(1, keepdim=True) * scale * 2.0 ** -31 * float(ks[pages, g].max())
+                weight = weight + 2.0 ** -12
+                seen = torch.where(hidden, 0.0, 1.0).to(v.dtype)
+                more = 2.0 ** -25 * p.amax(1, keepdim=True) * (seen @ v.abs()) + 2.0 ** -31 * float(vs[pages, g].max())
+            most = (p * size[:, g]).amax(1, keepdim=True)
+            seen_code = torch.where(hidden, 0.0, 1.0).to(v.dtype) @ code[:, g].abs()
+            bound[t, h] = (p @ v.abs()) * (weight + 2 * off) + 2.0 ** -25 * most * seen_code + more
+            lse_bound[t, h] = (math.log2(math.e) * (off + (2.0 ** -12 if chunk else 0) + 2.0 ** -20 + count * U32)).squeeze(1) \
+                + 4 * U32 * (1 + lse[t, h].abs())
     return o, lse, bound, lse_bound

@@ -211,8 +211,18 @@ def test_append_long_prompt(cuda_device):
 
 
 # --------------------------------------------------------------------------------------- attention
-def check_attention(o, lse, q, cache, table, lens, starts, scale):
-    ref, ref_lse, bound, lse_bound = paged64(q, *cache, table, lens, starts, scale)
+def takes_chunk_kernel(T, B, H, H_kv, D):
+    """The library's choice between its two kernels (csrc/fa_chunk.cu, use_chunk)."""
+    rows = -(-T * (H // H_kv) // B)
+    items = B * H_kv
+    waves = -(-items * -(-rows // 256) // 148)
+    return items * -(-rows // 16) >= (320 if D == 128 else 400) * waves
+
+
+def check_attention(o, lse, q, cache, table, lens, starts, scale, T=None):
+    """T: the call's query tokens, where q is only the ones that sequences have."""
+    chunk = takes_chunk_kernel(T or q.shape[0], len(lens), q.shape[1], cache[0].shape[1], q.shape[2])
+    ref, ref_lse, bound, lse_bound = paged64(q, *cache, table, lens, starts, scale, chunk)
     o = o.double().cpu()
     tol = half_step(q.dtype) * (ref.abs() + bound) + bound + half_subnormal(q.dtype)
     assert bool(o.isfinite().all())
@@ -256,6 +266,133 @@ def test_attention(lens, news, P, H, H_kv, D, dtype, cuda_device):
     assert torch.equal(o, _attend(*args, i32(starts)))  # the same bits every time
     if all(n == 1 for n in news):
         assert torch.equal(o, _attend(*args))
+
+
+CHUNKS = [
+    # lens, new tokens, page, H, H_kv, D: many rows, which the chunk kernel takes
+    ([700, 129, 128, 1], [500, 129, 100, 1], 64, 64, 16, 128),
+    ([5, 300, 0, 257], [50, 200, 0, 257], 16, 48, 16, 128),   # tokens in front of the first key, groups of 3
+    ([400, 383], [384, 129], 128, 28, 4, 128),                # groups of 7
+    ([333, 300], [333, 300], 32, 16, 16, 64),
+    ([1000], [256], 16, 32, 8, 64),
+    ([513, 640, 64], [300, 257, 64], 32, 40, 8, 32),
+    ([2100], [700], 64, 8, 8, 128),
+]
+
+
+@pytest.mark.parametrize("lens,news,P,H,H_kv,D", CHUNKS, ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_attention_of_many_rows(lens, news, P, H, H_kv, D, dtype, cuda_device):
+    table, starts, pages = batch(lens, news, P)
+    assert takes_chunk_kernel(starts[-1], len(lens), H, H_kv, D)
+    cache = make_cache(pages, H_kv, P, D)
+    q = (3 * torch.randn(starts[-1], H, D, generator=torch.Generator().manual_seed(5))).to(dtype)
+    gpu = _cache(*to_gpu(*cache))
+    args = (q.cuda(), gpu, table.cuda(), i32(lens), i32(starts))
+    o, lse = _attend(*args, return_lse=True)
+    _nat().check_status(cuda_device)
+    check_attention(o, lse, q, cache, table, lens, starts, D ** -0.5)
+    assert torch.equal(o, _attend(*args))
+
+
+def test_many_rows_read_only_what_they_see(cuda_device):
+    """The chunk kernel with NaN behind the last tokens, bad table entries behind the last pages, rows behind the last
+    sequence, strided q and out, and page scales of all sizes."""
+    P, H, H_kv, D = 32, 32, 16, 128
+    lens, news = [290, 33, 470, 3], [200, 33, 150, 9]
+    table, starts, pages = batch(lens, news, P, extra_pages=5)
+    kp, vp, ks, vs = make_cache(pages, H_kv, P, D)
+    vs *= torch.exp2(torch.randint(-30, 1, vs.shape, generator=torch.Generator().manual_seed(1)).float())
+    used = set()
+    for b, L in enumerate(lens):
+        for j in range(-(-L // P)):
+            page = int(table[b, j])
+            used.add(page)
+            for t in (kp, vp):
+                t.view(torch.uint8)[page, :, min(P, L - j * P):] = 0x7f
+    for page in set(range(pages)) - used:
+        ks[page] = vs[page] = float("nan")
+    T = starts[-1] + 5
+    assert takes_chunk_kernel(T, len(lens), H, H_kv, D)
+    q = torch.randn(T, H + 8, D, generator=torch.Generator().manual_seed(6)).bfloat16()
+    out = torch.full((T, 2 * H, D), 9.0, dtype=torch.bfloat16, device="cuda")
+    args = (q.cuda()[:, 8:], _cache(*to_gpu(kp, vp, ks, vs)), table.cuda(), i32(lens), i32(starts))
+    o, lse = _attend(*args, out=out[:, H:], return_lse=True)
+    _nat().check_status(cuda_device)
+    clean = [t.clone() for t in (kp, vp, ks, vs)]
+    for t in clean[:2]:
+        t.copy_(t.float().nan_to_num(0).to(E4M3))
+    n = starts[-1]
+    check_attention(o[:n], lse[:n], q[:n, 8:], clean, table, lens, starts, D ** -0.5, T)
+    assert bool((out[:, :H] == 9).all()) and bool((out[n:] == 9).all()) and bool((lse[n:] == -math.inf).all())
+    o2, lse2 = _attend(*args, return_lse=True)
+    assert torch.equal(o2[:n], o[:n]) and bool((o2[n:] == 0).all()) and torch.equal(lse2, lse)
+
+
+def test_many_rows_with_unusual_queries(cuda_device):
+    """bf16 queries far outside f16's range; NaN and infinity stay in their rows."""
+    P, H, H_kv, D = 64, 16, 16, 128
+    lens, news = [400, 380], [330, 360]
+    table, starts, pages = batch(lens, news, P)
+    cache = make_cache(pages, H_kv, P, D)
+    gpu = _cache(*to_gpu(*cache))
+    tables = (table.cuda(), i32(lens), i32(starts))
+    assert takes_chunk_kernel(starts[-1], 2, H, H_kv, D)
+    for power in (60, -60):
+        q = (torch.randn(starts[-1], H, D, generator=torch.Generator().manual_seed(1)) * 2.0 ** power).bfloat16()
+        o, lse = _attend(q.cuda(), gpu, *tables, scale=2.0 ** -power / 8, return_lse=True)
+        check_attention(o, lse, q, cache, table, lens, starts, 2.0 ** -power / 8)
+    q = torch.randn(starts[-1], H, D, generator=torch.Generator().manual_seed(1)).half()
+    ref = _attend(q.cuda(), gpu, *tables)
+    for bad in (float("nan"), float("inf")):
+        q2 = q.clone()
+        q2[5, 3, 7] = bad
+        o = _attend(q2.cuda(), gpu, *tables)
+        assert bool(o[5, 3].isnan().all())
+        keep = torch.ones(q.shape[:2], dtype=torch.bool)
+        keep[5, 3] = False
+        assert torch.equal(o.cpu()[keep], ref.cpu()[keep])
+
+
+def test_many_rows_failure_detection(cuda_device):
+    """A status word that is set stops the chunk kernel before it writes; in the failure-detection build, whose issuer
+    waits for something that never comes, it records a timeout and returns, and the product kernel works after that."""
+    import ctypes
+    import os
+    from tests.test_failure_detection_gpu import PIPELINE_TIMEOUT_CODES, STALL_LIB
+    from tests.test_serving_cpu import PAGED_ARGS
+    P, H, H_kv, D = 64, 16, 16, 128
+    lens, news = [400, 380], [330, 360]
+    table, starts, pages = batch(lens, news, P)
+    cache = make_cache(pages, H_kv, P, D)
+    tensors = to_gpu(*cache)
+    q = torch.randn(starts[-1], H, D, generator=torch.Generator().manual_seed(1)).half()
+    qg, tg, lg, sg = q.cuda(), table.cuda(), i32(lens), i32(starts)
+    nat = _nat()
+    status = nat.status_tensor(cuda_device)
+    out = torch.full_like(qg, 5.0)
+    status.fill_(1)
+    try:
+        _attend(qg, _cache(*tensors), tg, lg, sg, out=out)
+        torch.cuda.synchronize()
+        assert bool((out == 5).all())
+    finally:
+        status.zero_()
+    if not os.path.exists(STALL_LIB):
+        pytest.skip("the failure-detection build is not there")
+    lib = ctypes.CDLL(STALL_LIB)
+    own = torch.zeros(4, dtype=torch.int32, device="cuda")
+    workspace = torch.empty(16 << 20, dtype=torch.uint8, device="cuda")
+    packed = PAGED_ARGS.pack(qg.data_ptr(), *(t.data_ptr() for t in tensors), tg.data_ptr(), lg.data_ptr(), sg.data_ptr(),
+                             out.data_ptr(), 0, workspace.data_ptr(), H * D, D, H * D, D, tg.stride(0), starts[-1], 2, tg.shape[1],
+                             pages, H, H_kv, P, D, 0, 0, D ** -0.5)
+    lib.fa_paged_attention.argtypes = [ctypes.c_void_p] * 3
+    assert lib.fa_paged_attention(packed, own.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert own.tolist()[0] in PIPELINE_TIMEOUT_CODES
+    o = _attend(qg, _cache(*tensors), tg, lg, sg)
+    nat.check_status(cuda_device)
+    check_attention(o, None, q, cache, table, lens, starts, D ** -0.5)
 
 
 def test_attention_reads_only_what_it_sees(cuda_device):
