@@ -44,11 +44,13 @@ constexpr int kBN = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kLaunchRegs = 128;
-constexpr int kRegsSoftmax = 192;
-constexpr int kRegsOther = 64;
+constexpr int kRegsSoftmax = 184;
+constexpr int kRegsOther = 72;
 static_assert(256 * kRegsOther + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split");
 constexpr int kSoftmaxCopy = 1;  // the softmax warpgroups' own copy of the bounded-wait loop
-constexpr int kPolyPairs = 4;    // of 16 exp2 pairs on interior tiles: the dense forward's share
+// Of 16 exp2 pairs on interior tiles, those on the FMA pipe.  The conversions share that pipe's issue slots, so fewer
+// pay than in the dense forward: 3 x 1024 tokens behind 8192 keys take 290 us with one, 298 with two, 311 with four.
+constexpr int kPolyPairs = 1;
 constexpr float kHeadroom = 64.f;  // f16(448 * 64) is finite
 
 template <int D>
