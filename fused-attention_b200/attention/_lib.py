@@ -228,7 +228,11 @@ def _status_for_ops(idx, only_ask):
     """The status word of device idx for the native torch binding: its address, or whether it is there."""
     if only_ask:
         return idx in _status
-    return status_tensor(torch.device("cuda", idx)).data_ptr()
+    new = idx not in _status
+    word = status_tensor(torch.device("cuda", idx)).data_ptr()
+    if new:
+        torch.cuda.current_stream(idx).synchronize()  # zeroed before a call on any stream reads it
+    return word
 
 
 def load_ops():

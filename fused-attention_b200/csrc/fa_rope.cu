@@ -453,9 +453,10 @@ cudaError_t launch_rope_bwd(RopeParams p, int D, bool bf16, bool interleaved, cu
   const long long k_units = token_blocks * ((p.H_kv + p.range_heads - 1) / p.range_heads);
   // one wave of blocks, shared out by the number of heads
   const long long k_share = p.H_kv == 0 ? 0 : (kRopeBwdBlocks * static_cast<long long>(p.H_kv) + p.H + p.H_kv - 1) / (p.H + p.H_kv);
-  const long long q_share = kRopeBwdBlocks - k_share;
+  const long long k_most = k_share < kRopeBwdBlocks ? k_share : kRopeBwdBlocks - 1;  // the queries keep one
+  const long long q_share = kRopeBwdBlocks - k_most;
   p.q_blocks = static_cast<int>(q_units < q_share ? q_units : q_share);
-  const int blocks = p.q_blocks + static_cast<int>(k_units < k_share ? k_units : k_share);
+  const int blocks = p.q_blocks + static_cast<int>(k_units < k_most ? k_units : k_most);
 #define FA_ROPE_CASE(DD, BB, II)                                  \
   if (D == DD && bf16 == BB && interleaved == II)                 \
     rope_bwd_kernel<DD, BB, II><<<blocks, kRopeThreads, 0, stream>>>(p);

@@ -48,8 +48,8 @@ int check_cache(int B, int T, int width, int num_pages, int H_kv, int page_size,
   if (offsets == nullptr && T != B) return FA_ERR_INVALID_ARG;
   if (!head_dim_ok(D) || (dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_BF16)) return FA_ERR_UNSUPPORTED;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FA_ERR_UNSUPPORTED;
-  // lengths and row indexes are 32-bit inside the kernels
-  if (static_cast<long long>(width) * page_size > (1LL << 30) || H_kv > 65535 || T > (1 << 28)) return FA_ERR_UNSUPPORTED;
+  // lengths and row indexes are 32-bit inside the kernels, and 2 H_kv is a grid dimension
+  if (static_cast<long long>(width) * page_size > (1LL << 30) || H_kv > 32767 || T > (1 << 28)) return FA_ERR_UNSUPPORTED;
   if (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(k_scales, 4) || !aligned(v_scales, 4) ||
       !aligned(table, 4) || !aligned(seq_lens, 4) || !aligned(offsets, 4))
     return FA_ERR_ALIGNMENT;
@@ -149,7 +149,7 @@ int fa_append_kv(const fa_append_args* a, int* dev_status, void* stream) {
     if ((rc = check_axes(a->axes, a->section_start, a->D, a->max_pos, p.section_start)) != FA_OK) return rc;
     if (a->axes > 1 && a->pos == nullptr) return FA_ERR_INVALID_ARG;
   }
-  if (!aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cos, 4) || !aligned(a->sin, 4) ||
+  if (!aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cos, 16) || !aligned(a->sin, 16) ||
       !aligned(a->pos, a->pos_is_int64 ? 8 : 4) || !strides_ok(a->k_stride) || !strides_ok(a->v_stride))
     return FA_ERR_ALIGNMENT;
   if ((rc = fa::check_device()) != FA_OK) return rc;

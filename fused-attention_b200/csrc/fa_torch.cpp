@@ -432,7 +432,8 @@ py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, 
   if (T > 0 && B > 0) {
     fa_paged_args a{};
     const Tensor qr = rows(q, a.q_stride);
-    TORCH_CHECK_VALUE(row_strides(out, a.out_stride), "out must be contiguous in D with its base and strides on 16-byte boundaries");
+    TORCH_CHECK_VALUE(row_strides(out, a.out_stride) && (T == 1 || a.out_stride[0] != 0) && (H == 1 || a.out_stride[1] != 0),
+                      "out must be contiguous in D, with its base and strides on 16-byte boundaries, and not expanded");
     const Tensor workspace = at::empty({FA_PAGED_WORKSPACE_BYTES(D)}, q.options().dtype(at::kByte));
     a.q = qr.const_data_ptr();
     a.k_pages = kp.const_data_ptr();

@@ -184,7 +184,7 @@ FA_API int fa_append_kv(const struct fa_append_args* args, int* dev_status, void
 #define FA_PAGED_WORKSPACE_BYTES(D) (75776LL * (D) + 196608)
 
 /* Attention of T query tokens ([T, H, D]) over the cache: query token i of sequence b's n new tokens
- * sees its keys j <= seq_lens[b] - n + i.  out [T, H, D]; lse [T, H] (log2 domain) or NULL; a row
+ * sees its keys j <= seq_lens[b] - n + i.  Scales are finite and not negative.  out [T, H, D]; lse [T, H] (log2 domain) or NULL; a row
  * that sees no key gets 0 and -inf. */
 struct fa_paged_args {
   const void* q;

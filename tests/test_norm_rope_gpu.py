@@ -156,6 +156,18 @@ def test_rows_of_zeros_and_extremes(cuda_device):
         assert torch.equal(got[0, keep], ref[0, keep])
 
 
+def test_far_more_key_heads_than_query_heads(cuda_device):
+    """The backward blocks are shared out by heads: the queries keep some however few heads they have."""
+    q, k, cos, sin, pos, w, _, dz = make(1, 1, 400, 3, 32, torch.float16, torch.float32)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, *w)]
+    out = _op()(leaves[0], leaves[1], cos, sin, pos, leaves[2], leaves[3])
+    grads = torch.autograd.grad(out, leaves, dz)
+    c, s = (x.unsqueeze(1) for x in angles(cos, sin, pos, None))
+    with torch.no_grad():
+        check_backward(grads[0], grads[2], q, w[0], c, s, False, dz[0], "q")
+        check_backward(grads[1], grads[3], k, w[1], c, s, False, dz[1], "k")
+
+
 @pytest.mark.parametrize("N", [0, 1])
 def test_lengths_zero_and_one(N, cuda_device):
     q, k, cos, sin, pos, w, _, _ = make(2, 3, 1, N, 64, torch.float16, torch.float32)
@@ -240,8 +252,7 @@ def test_same_bits_every_time_and_many_blocks(cuda_device):
 
 
 def test_streams_and_graphs(cuda_device):
-    """Another stream than the inputs', and a captured forward and backward replayed on new inputs while an
-    uncaptured graph of other leaves is alive."""
+    """Another stream than the inputs', and a captured forward and backward replayed on new inputs."""
     q, k, cos, sin, pos, w, _, dz = make(2, 4, 2, 40, 64, torch.bfloat16, torch.bfloat16, fused=False)
     ref = _op()(q, k, cos, sin, pos, *w)
     side = torch.cuda.Stream()

@@ -531,6 +531,32 @@ def test_many_sequences_and_long_tables(cuda_device):
     check_attention(o, lse, q, cache, table, lens, starts, D ** -0.5)
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("group,n", [(4, 1), (16, 1), (3, 7)])
+def test_full_grids_fit_the_workspace(D, group, n, cuda_device):
+    """Tables wide enough for a full grid of blocks, with both row tiles: every block has its part of the workspace."""
+    P, H_kv = 16, 4
+    lens = [900, 20, 333, 5, 700, 64]
+    news = [min(n, L) for L in lens]
+    table, starts, pages = batch(lens, news, P, width=2000)
+    cache = make_cache(pages, H_kv, P, D)
+    q = torch.randn(starts[-1], H_kv * group, D, generator=torch.Generator().manual_seed(3)).half()
+    o, lse = _attend(q.cuda(), _cache(*to_gpu(*cache)), table.cuda(), i32(lens), i32(starts), return_lse=True)
+    _nat().check_status(cuda_device)
+    check_attention(o, lse, q, cache, table, lens, starts, D ** -0.5)
+
+
+def test_out_that_overlaps_itself_is_refused(cuda_device):
+    P, H, H_kv, D = 16, 4, 2, 64
+    table, starts, pages = batch([40, 20], [1, 1], P)
+    gpu = _cache(*to_gpu(*make_cache(pages, H_kv, P, D)))
+    q = torch.randn(2, H, D, device="cuda").half()
+    for out in (torch.empty(1, H, D, device="cuda").half().expand(2, H, D), torch.empty(2, 1, D, device="cuda").half().expand(2, H, D),
+                torch.empty(2, D, H, device="cuda").half().transpose(1, 2)):
+        with pytest.raises(ValueError, match="out must be contiguous"):
+            _attend(q, gpu, table.cuda(), i32([40, 20]), out=out)
+
+
 def test_cache_past_32_bit_offsets(cuda_device):
     """Pages whose byte offsets pass 2^32."""
     P, H, H_kv, D = 128, 8, 2, 128

@@ -227,7 +227,8 @@ CACHE_CODES = [
 
 @pytest.mark.parametrize("kw,code", CACHE_CODES + [
     (dict(k=0), 1), (dict(cos=256), 1), (dict(cos=256, sin=256), 1), (dict(cos=256, sin=256, max_pos=4, axes=2, s1=8), 1),
-    (dict(kw=256, wdtype=1), 2), (dict(kw=264), 3), (dict(v=260), 3)])
+    (dict(kw=256, wdtype=1), 2), (dict(kw=264), 3), (dict(v=260), 3), (dict(cos=264, sin=256, max_pos=4), 3),
+    (dict(H_kv=32768), 2)])
 def test_append_c_refusals(kw, code):
     if kw.get("st", 0) is None:
         kw = dict(st=[4] + [64] * 5)
