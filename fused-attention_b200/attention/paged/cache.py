@@ -76,7 +76,7 @@ def append_kv(cache, k, v, block_table, seq_lens, offsets=None, cos=None, sin=No
     k, v:         [T, H_kv, D] float16 / bfloat16 (any strides with a contiguous last dimension)
     block_table:  int32 [B, pages], the pages of each sequence
     seq_lens:     int32 [B], lengths with the new tokens
-    offsets:      int32 [B + 1], sequence b's new tokens are k[offsets[b]:offsets[b + 1]], the last ones of
+    offsets:      int32 [B + 1] from 0, sequence b's new tokens are k[offsets[b]:offsets[b + 1]], the last ones of
                   its seq_lens[b]; None: one token per sequence
     cos, sin:     float32 [max_pos, D/2]: keys are rotated by their position, which is their place in the
                   sequence unless positions (int32 / int64 [T], with sections [axes, T]) says otherwise
@@ -84,8 +84,8 @@ def append_kv(cache, k, v, block_table, seq_lens, offsets=None, cos=None, sin=No
 
     The tokens of one call that lie in one page are rounded together, to the smallest power-of-two scale
     that holds them; a page that holds older tokens keeps its scale unless the new ones need a larger
-    one, and then the older ones are rounded again.  Infinities are stored as the largest magnitude, NaN
-    as NaN; neither changes a scale.  Tokens behind offsets[B], and tokens that would lie before their
+    one, and then the older ones are rounded again.  Infinities in v, and in k where it is neither normed nor
+    rotated, are stored as the largest magnitude, NaN as NaN; neither changes a scale.  Tokens behind offsets[B], and tokens that would lie before their
     sequence's start, are not written.  A page that is written must belong to one sequence of the batch.
     """
     (_ops or _load_ops()).append_kv(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, k, v, block_table, seq_lens,
