@@ -142,6 +142,8 @@ __device__ __forceinline__ void issue_pv_half(uint32_t o_tmem, uint32_t p_tmem, 
   }
 }
 
+constexpr int kNanWord = 6;  // words[kNanWord]: a value that some row may not see is NaN
+
 struct ChunkWork {
   int b, h;       // sequence, K/V head; b < 0: nothing to do
   int first, n;   // flat index of the sequence's first new token, their number
@@ -156,7 +158,10 @@ __device__ __forceinline__ ChunkWork find_work(const PagedParams& p, int* words)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int chunk = (p.B + kThreads - 1) / kThreads;
   const int b0 = min(p.B, static_cast<int>(threadIdx.x) * chunk), b1 = min(p.B, b0 + chunk);
-  if (threadIdx.x == 0) words[0] = -1;
+  if (threadIdx.x == 0) {
+    words[0] = -1;
+    words[kNanWord] = 0;
+  }
   long long mine = 0;
   int first = 0, n = 0, len = 0;
   auto shape = [&](int b) {
@@ -300,6 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
   const int nkv1 = ntiles == 2 ? (max(1, keys_of(1)) + kBN - 1) / kBN : 0;
   const int nmax = max(nkv0, nkv1);
   const uint32_t sK = base + C::kOffK, sV = base + C::kOffV;
+  // the first key tile that some row of the block does not see to its end
+  const int first_hidden = max(0, w.before + w.r0 / p.group + 1) / kBN;
 
   if (warp >= kSoftmaxWarps) {
     regs_decrease<kRegsOther>();
@@ -377,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       uint8_t* ring = smem + (is_k ? C::kOffK : C::kOffV);
       // A block's bytes wait in shared memory (asynchronous copies, each thread its own pieces) from the
       // moment the block of the tile before has been converted: nearly a tile's time in flight.
-      const uint8_t* raw = smem + C::kOffRaw + (is_k ? 0 : 128 * D) + first_block * 16 * D + lane * 16;
+      uint8_t* raw = smem + C::kOffRaw + (is_k ? 0 : 128 * D) + first_block * 16 * D + lane * 16;
       const uint32_t full = BAR(is_k ? BAR_KFULL : BAR_VFULL), empty = BAR(is_k ? BAR_KEMPTY : BAR_VEMPTY);
       const uint32_t page_bytes = static_cast<uint32_t>(D) << p.page_shift;
       const int page_mask = (1 << p.page_shift) - 1;
@@ -410,10 +417,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       for (int blk = 0; blk < kMost; ++blk)
         if (blk < blocks) copy(0, blk);
       bool ok = true;
-      for (int j = 0; ok && j < nmax; ++j) {
+      auto convert_tile = [&](int j, auto clean) {
         const int st = j % ST;
         uint8_t* tile = ring + st * C::kTileBytes;
-        if (!(ok = mbar_wait(empty + 8 * st, ((j / ST) & 1) ^ 1, p.status, kDevTimeoutKVEmpty))) break;
+        if (!(ok = mbar_wait(empty + 8 * st, ((j / ST) & 1) ^ 1, p.status, kDevTimeoutKVEmpty))) return;
 #pragma unroll
         for (int blk = 0; blk < kMost; ++blk) {
           if (blk < blocks) {
@@ -427,6 +434,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
             const __half2 f2h = __float2half2_rn(small ? relative * (1.f / kSmall) : relative);
             const uint32_t factor = *reinterpret_cast<const uint32_t*>(&f2h);
             const int row0 = (first_block + blk) * 16 + row_in_block;
+            if constexpr (decltype(clean)::value) {
+#pragma unroll 1
+              for (int i = 0; i < kLoads; ++i) {
+                uint4* piece_at = reinterpret_cast<uint4*>(raw + blk * 16 * D + i * 512);
+                const uint4 v = *piece_at;
+                const uint4 nan = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
+                if ((nan.x | nan.y | nan.z | nan.w) != 0) {
+                  if (j * kBN + row0 + i * kRowsPerLoad < keys) *const_cast<volatile int*>(&words[kNanWord]) = 1;
+                  *piece_at = make_uint4(v.x & ~nan.x, v.y & ~nan.y, v.z & ~nan.z, v.w & ~nan.w);
+                }
+              }
+            }
             auto convert = [&](auto is_small) {
 #pragma unroll
               for (int i = 0; i < kLoads; ++i) {
@@ -451,7 +470,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
         }
         fence_async_shared();
         mbar_arrive(full + 8 * st);
-      }
+      };
+      // Values that some row does not see: NaN is taken out (0 * NaN is not 0) and put back at the end.  A loop of
+      // its own: inside the common one the same lines cost 8 % of the kernel.
+      const int plain = is_k ? nmax : min(nmax, first_hidden);
+      int j = 0;
+      for (; ok && j < plain; ++j) convert_tile(j, std::false_type{});
+      for (; ok && j < nmax; ++j) convert_tile(j, std::true_type{});
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
     }
@@ -607,11 +632,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
         const bool seen = own_last >= 0;
         const float f = seen ? (top_v / kHeadroom) / l : 0.f;
         uint16_t* out = static_cast<uint16_t*>(p.out) + token * p.out_stride[0] + head * p.out_stride[1];
+        const bool nan = *const_cast<volatile int*>(&words[kNanWord]) != 0;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
           tmem_ld_wait(o);
+          if (nan && live) {  // rare: the values that were NaN among the keys that the row sees
+            for (int key = first_hidden * kBN; key <= own_last; ++key) {
+              const int page = table[key >> p.page_shift];
+              if (page < 0 || page >= p.num_pages) continue;
+              const uint32_t* row = reinterpret_cast<const uint32_t*>(
+                  p.v_pages + (((static_cast<size_t>(page) * p.H_kv + w.h) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D + c * 32);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if ((nan_bytes(row[i / 4]) >> (8 * (i % 4)) & 1u) != 0) o[i] = 0x7fffffffu;
+            }
+          }
           if (live) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {

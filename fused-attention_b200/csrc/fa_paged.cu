@@ -238,10 +238,13 @@ struct WarpState {
   float l[NT][2];           // this thread's sum of 2^(s - m)
 };
 
+// EDGE: keys behind a row's last are masked, V's bytes behind the tile's last key are cleared, and so is NaN in V,
+// which sets *saw_nan: the caller puts it back for the rows that see it.
 template <int D, int NT, bool EDGE>
 __device__ __forceinline__ void softmax_pv(WarpState<D, NT>& st, float (&s)[NT][2][4], const float (&qs)[NT][2],
                                            const float (&ks)[2], const float (&vs)[2], VBlock<D> (&v)[2],
-                                           const int (&last)[NT][2], int key0, int keys, int g, int t) {
+                                           const int (&last)[NT][2], int key0, int keys, int g, int t,
+                                           volatile int* saw_nan) {
   bool raise = false;
   float top[NT][2][2];  // per column: this thread's largest score, and with its page's scale
 #pragma unroll
@@ -315,12 +318,20 @@ __device__ __forceinline__ void softmax_pv(WarpState<D, NT>& st, float (&s)[NT][
   }
 #pragma unroll
   for (int blk = 0; blk < 2; ++blk) {
-    if (EDGE) {  // bytes behind the last key may hold anything, NaN too: 0 * NaN is not 0
+    if (EDGE) {  // bytes behind the last key may hold anything: 0 * NaN is not 0
+      uint32_t nan = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (key0 + 16 * blk + 2 * t + (i & 1) + 8 * (i >> 1) >= keys)
+      for (int i = 0; i < 4; ++i) {
+        const bool behind = key0 + 16 * blk + 2 * t + (i & 1) + 8 * (i >> 1) >= keys;
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) v[blk].w[i][w] = 0;
+        for (int w = 0; w < D / 32; ++w) {
+          if (behind) v[blk].w[i][w] = 0;
+          const uint32_t mask = nan_bytes(v[blk].w[i][w]);
+          v[blk].w[i][w] &= ~mask;
+          nan |= mask;
+        }
+      }
+      if (nan != 0) *saw_nan = 1;
     }
 #pragma unroll
     for (int w = 0; w < D / 32; ++w)
@@ -342,6 +353,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
   constexpr int RT = 8 * NT;
   __shared__ float sh_o[kWarps][RT][D + 4];  // +4: rows start on different banks
   __shared__ float sh_m[kWarps][RT], sh_l[kWarps][RT];
+  __shared__ volatile int sh_nan[kWarps];  // the warp met NaN in a value that some row does not see
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int g = lane / 4, t = lane % 4;
@@ -452,6 +464,8 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
       return page;
     };
     int key0 = u0 * kUnit + warp * kTile;
+    if (lane == 0) sh_nan[warp] = 0;
+    __syncwarp();
     if (key0 < key_end) {
       KBlock<D> k[2];
       size_t at[2];     // (page, head) of the tile's two blocks
@@ -506,9 +520,9 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
         vs[0] = __log2f(vs[0]);
         vs[1] = __log2f(vs[1]);
         if (key0 + kTile > seen_by_all)
-          softmax_pv<D, NT, true>(st, s, qs, ks, vs, v, last, key0, keys, g, t);
+          softmax_pv<D, NT, true>(st, s, qs, ks, vs, v, last, key0, keys, g, t, &sh_nan[warp]);
         else
-          softmax_pv<D, NT, false>(st, s, qs, ks, vs, v, last, key0, keys, g, t);
+          softmax_pv<D, NT, false>(st, s, qs, ks, vs, v, last, key0, keys, g, t, &sh_nan[warp]);
         if (!more) break;
         key0 = key_next;
         key_next += kWarps * kTile;
@@ -545,6 +559,24 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
           *reinterpret_cast<float4*>(row + 2 * mt) = make_float4(st.o[nt][mt][c], st.o[nt][mt][2 + c],
                                                                  st.o[nt][mt + 1][c], st.o[nt][mt + 1][2 + c]);
       }
+    __syncwarp();
+    if (sh_nan[warp] != 0) {  // rare: NaN among the values that some row does not see, for those that do
+#pragma unroll 1
+      for (int k0 = u0 * kUnit + warp * kTile; k0 < key_end; k0 += kWarps * kTile) {
+        if (k0 + kTile <= seen_by_all) continue;
+#pragma unroll 1
+        for (int key = k0; key < min(k0 + kTile, keys); ++key) {
+          const uint8_t* row = p.v_pages + (static_cast<size_t>(page_of(key)) * p.H_kv + h) * kv_head_bytes +
+                               (key & page_mask) * D;
+#pragma unroll 1
+          for (int d = lane; d < D; d += 32)
+            if ((row[d] & 0x7f) == 0x7f)
+#pragma unroll 1
+              for (int r = 0; r < RT; ++r)
+                if (key <= before + (r0 + r) / p.group) sh_o[warp][r][d] = __int_as_float(0x7fffffff);
+        }
+      }
+    }
     __syncthreads();
     const bool whole = u0 == 0 && u1 == per_tile;
     const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);

@@ -6,6 +6,11 @@
 
 namespace fa {
 
+// The bytes of w that are NaN in e4m3 (0x7f, 0xff), as a mask of whole bytes.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+}
+
 // Output rows of tokens that no sequence has: o = 0, lse = -inf.  The grid's blocks share them; usually there are none.
 template <int D>
 __device__ __forceinline__ void clear_unowned_rows(const PagedParams& p) {

@@ -531,6 +531,57 @@ def test_many_sequences_and_long_tables(cuda_device):
     check_attention(o, lse, q, cache, table, lens, starts, D ** -0.5)
 
 
+def nan_case(lens, news, P, H, H_kv, D, dtype):
+    """NaN values among the new tokens' keys, hidden from the tokens before them: (q, tensors, clean tensors, the
+    entries of o that have to be NaN, table, starts)."""
+    table, starts, pages = batch(lens, news, P)
+    kp, vp, ks, vs = make_cache(pages, H_kv, P, D)
+    g = torch.Generator().manual_seed(9)
+    expected = torch.zeros(starts[-1], H, D, dtype=torch.bool)
+    clean = vp.clone()
+    for b, (L, n) in enumerate(zip(lens, news)):
+        for _ in range(3):
+            key = L - 1 - int(torch.randint(0, max(1, min(n, L)), (), generator=g))
+            head, d = int(torch.randint(0, H_kv, (), generator=g)), int(torch.randint(0, D, (), generator=g))
+            page = int(table[b, key // P])
+            vp.view(torch.uint8)[page, head, key % P, d] = 0xff if d % 2 else 0x7f
+            clean.view(torch.uint8)[page, head, key % P, d] = 0
+            for i in range(n):
+                if L - n + i >= key:
+                    expected[starts[b] + i, head * (H // H_kv):(head + 1) * (H // H_kv), d] = True
+    q = torch.randn(starts[-1], H, D, generator=g).to(dtype)
+    return q, (kp, vp, ks, vs), (kp, clean, ks, vs), expected, table, starts
+
+
+@pytest.mark.parametrize("lens,news,P,H,H_kv,D", [
+    ([50, 133], [5, 40], 16, 8, 2, 64), ([300, 40], [20, 9], 64, 4, 4, 128), ([90], [60], 32, 6, 1, 32),
+    ([700, 129, 128], [500, 129, 100], 64, 64, 16, 128), ([333, 300], [333, 300], 32, 16, 16, 64),
+    ([513, 640, 64], [300, 257, 64], 32, 40, 8, 32)], ids=str)
+def test_nan_values_reach_only_the_tokens_that_see_them(lens, news, P, H, H_kv, D, cuda_device):
+    q, tensors, clean, expected, table, starts = nan_case(lens, news, P, H, H_kv, D, torch.float16)
+    o = _attend(q.cuda(), _cache(*to_gpu(*tensors)), table.cuda(), i32(lens), i32(starts))
+    _nat().check_status(cuda_device)
+    o = o.cpu()
+    assert torch.equal(o.isnan(), expected)
+    ref = _attend(q.cuda(), _cache(*to_gpu(*clean)), table.cuda(), i32(lens), i32(starts)).cpu()
+    assert torch.equal(o[~expected], ref[~expected])
+
+
+def test_nan_keys_reach_only_the_tokens_that_see_them(cuda_device):
+    for lens, news, P, H, H_kv, D in (([50, 133], [5, 40], 16, 8, 2, 64), ([700, 129, 128], [500, 129, 100], 64, 64, 16, 128)):
+        table, starts, pages = batch(lens, news, P)
+        kp, vp, ks, vs = make_cache(pages, H_kv, P, D)
+        q = torch.randn(starts[-1], H, D, generator=torch.Generator().manual_seed(1)).half()
+        args = (table.cuda(), i32(lens), i32(starts))
+        ref = _attend(q.cuda(), _cache(*to_gpu(kp, vp, ks, vs)), *args).cpu()
+        key = lens[0] - 3
+        kp.view(torch.uint8)[int(table[0, key // P]), 1, key % P, 5] = 0x7f
+        o = _attend(q.cuda(), _cache(*to_gpu(kp, vp, ks, vs)), *args).cpu()
+        hit = torch.zeros(o.shape[:2], dtype=torch.bool)
+        hit[starts[1] - 3:starts[1], H // H_kv:2 * (H // H_kv)] = True
+        assert bool(o[hit].isnan().all()) and torch.equal(o[~hit], ref[~hit])
+
+
 @pytest.mark.parametrize("D", [32, 64, 128])
 @pytest.mark.parametrize("group,n", [(4, 1), (16, 1), (3, 7)])
 def test_full_grids_fit_the_workspace(D, group, n, cuda_device):
