@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       uint8_t* ring = smem + (is_k ? C::kOffK : C::kOffV);
       // A block's bytes wait in shared memory (asynchronous copies, each thread its own pieces) from the
       // moment the block of the tile before has been converted: nearly a tile's time in flight.
-      uint8_t* raw = smem + C::kOffRaw + (is_k ? 0 : 128 * D) + first_block * 16 * D + lane * 16;
+      const uint8_t* raw = smem + C::kOffRaw + (is_k ? 0 : 128 * D) + first_block * 16 * D + lane * 16;
       const uint32_t full = BAR(is_k ? BAR_KFULL : BAR_VFULL), empty = BAR(is_k ? BAR_KEMPTY : BAR_VEMPTY);
       const uint32_t page_bytes = static_cast<uint32_t>(D) << p.page_shift;
       const int page_mask = (1 << p.page_shift) - 1;
@@ -434,24 +434,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
             const __half2 f2h = __float2half2_rn(small ? relative * (1.f / kSmall) : relative);
             const uint32_t factor = *reinterpret_cast<const uint32_t*>(&f2h);
             const int row0 = (first_block + blk) * 16 + row_in_block;
-            if constexpr (decltype(clean)::value) {
-#pragma unroll 1
-              for (int i = 0; i < kLoads; ++i) {
-                uint4* piece_at = reinterpret_cast<uint4*>(raw + blk * 16 * D + i * 512);
-                const uint4 v = *piece_at;
-                const uint4 nan = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
-                if ((nan.x | nan.y | nan.z | nan.w) != 0) {
-                  if (j * kBN + row0 + i * kRowsPerLoad < keys) *const_cast<volatile int*>(&words[kNanWord]) = 1;
-                  *piece_at = make_uint4(v.x & ~nan.x, v.y & ~nan.y, v.z & ~nan.z, v.w & ~nan.w);
-                }
-              }
-            }
             auto convert = [&](auto is_small) {
 #pragma unroll
               for (int i = 0; i < kLoads; ++i) {
                 const int row = row0 + i * kRowsPerLoad;
                 uint4 v = *reinterpret_cast<const uint4*>(raw + blk * 16 * D + i * 512);
                 if (j * kBN + row >= keys) v = make_uint4(0, 0, 0, 0);  // behind the last key
+                if constexpr (decltype(clean)::value) {
+                  const uint4 nan = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
+                  if ((nan.x | nan.y | nan.z | nan.w) != 0) *const_cast<volatile int*>(&words[kNanWord]) = 1;
+                  v = make_uint4(v.x & ~nan.x, v.y & ~nan.y, v.z & ~nan.z, v.w & ~nan.w);
+                }
                 uint4 lo, hi;
                 dequant16<decltype(is_small)::value>(v, factor, lo, hi);
                 // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes
