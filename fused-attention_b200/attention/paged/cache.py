@@ -38,7 +38,7 @@ def _load_ops():
 class PagedKVCache:
     """The cache's four tensors: k_pages, v_pages (torch.float8_e4m3fn [num_pages, H_kv, page_size, D], page_size 16,
     32, 64 or 128, D 32, 64 or 128) and k_scales, v_scales (float32 [num_pages, H_kv]), all contiguous on one
-    device.  The operators write into these tensors."""
+    device; appending needs keys and values that share no memory.  The operators write into these tensors."""
 
     __slots__ = ("k_pages", "v_pages", "k_scales", "v_scales")
 
@@ -85,8 +85,8 @@ def append_kv(cache, k, v, block_table, seq_lens, offsets=None, cos=None, sin=No
     The tokens of one call that lie in one page are rounded together, to the smallest power-of-two scale
     that holds them; a page that holds older tokens keeps its scale unless the new ones need a larger
     one, and then the older ones are rounded again.  Infinities in v, and in k where it is neither normed nor
-    rotated, are stored as the largest magnitude, NaN as NaN; neither changes a scale.  Tokens behind offsets[B], and tokens that would lie before their
-    sequence's start, are not written.  A page that is written must belong to one sequence of the batch.
+    rotated, are stored as the largest magnitude, NaN as NaN; neither changes a scale.  Tokens behind
+    offsets[B], and tokens that would lie before their sequence's start, are not written.  A page that is written must belong to one sequence of the batch.
     """
     (_ops or _load_ops()).append_kv(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, k, v, block_table, seq_lens,
                                     offsets, cos, sin, positions, k_weight, eps, interleaved, sections)

@@ -10,6 +10,11 @@ namespace {
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+bool overlap(const void* a, const void* b, size_t bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return (x < y ? y - x : x - y) < bytes;
+}
+
 bool head_dim_ok(int D) { return D == 32 || D == 64 || D == 128; }
 
 int page_shift(int page_size) { return page_size == 16 ? 4 : (page_size == 32 ? 5 : (page_size == 64 ? 6 : 7)); }
@@ -152,6 +157,10 @@ int fa_append_kv(const fa_append_args* a, int* dev_status, void* stream) {
   if (!aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->cos, 16) || !aligned(a->sin, 16) ||
       !aligned(a->pos, a->pos_is_int64 ? 8 : 4) || !strides_ok(a->k_stride) || !strides_ok(a->v_stride))
     return FA_ERR_ALIGNMENT;
+  // keys and values are written at the same time
+  const size_t slots = static_cast<size_t>(a->num_pages) * a->H_kv;
+  if (overlap(a->k_pages, a->v_pages, slots * a->page_size * a->D) || overlap(a->k_scales, a->v_scales, slots * sizeof(float)))
+    return FA_ERR_INVALID_ARG;
   if ((rc = fa::check_device()) != FA_OK) return rc;
   p.k = a->k;
   p.v = a->v;

@@ -353,6 +353,11 @@ void append_kv(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tenso
                   !(k.requires_grad() || v.requires_grad() || (k_weight.has_value() && k_weight->requires_grad())),
               "append_kv has no backward: call it under torch.no_grad()");
   check_cache(kp, vp, ks, vs);
+  auto apart = [](const Tensor& x, const Tensor& y) {
+    const uintptr_t i = reinterpret_cast<uintptr_t>(x.const_data_ptr()), j = reinterpret_cast<uintptr_t>(y.const_data_ptr());
+    return (i < j ? j - i : i - j) >= x.nbytes();
+  };
+  TORCH_CHECK_VALUE(apart(kp, vp) && apart(ks, vs), "append_kv writes keys and values: their pages and scales must not share memory");
   const int64_t H_kv = kp.size(1), D = kp.size(3);
   TORCH_CHECK_VALUE(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == H_kv && k.size(2) == D, "k, v must be (T, H_kv=", H_kv,
                     ", D=", D, "); got ", k.sizes(), ", ", v.sizes());

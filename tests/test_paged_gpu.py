@@ -516,6 +516,20 @@ def test_strides_and_shared_pages(cuda_device):
     assert torch.equal(_attend(odd, _cache(*to_gpu(*cache)), table.cuda(), i32(lens)), o)
 
 
+@pytest.mark.parametrize("lens,news,P,H,H_kv,D", [ATTENDS[2], ATTENDS[8], CHUNKS[0], CHUNKS[3]], ids=str)
+def test_out_may_be_q_and_keys_may_be_values(lens, news, P, H, H_kv, D, cuda_device):
+    """Writing o over q, and a cache whose keys are its values: the same bits as apart."""
+    table, starts, pages = batch(lens, news, P)
+    kp, vp, ks, vs = make_cache(pages, H_kv, P, D)
+    q = torch.randn(starts[-1], H, D, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    args = (table.cuda(), i32(lens), i32(starts))
+    apart = _attend(q, _cache(*to_gpu(kp, kp.clone(), ks, ks.clone())), *args)
+    kg, sg = to_gpu(kp, vp, ks, vs)[::2]
+    o = q.clone()
+    assert _attend(o, _cache(kg, kg, sg, sg), *args, out=o) is o
+    assert torch.equal(o, apart)
+
+
 def test_many_sequences_and_long_tables(cuda_device):
     """More sequences than a block has threads, most of them short, one long; a table much wider than needed."""
     P, H, H_kv, D = 16, 4, 2, 32

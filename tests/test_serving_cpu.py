@@ -134,6 +134,17 @@ def test_append_refuses(kw, error, match):
         append_kv(**step_args(**a))
 
 
+def test_append_refuses_keys_and_values_in_one_place():
+    """Attention may read a cache whose keys are its values; an append would write both."""
+    kp, vp, ks, vs = cache_tensors()
+    both = torch.zeros(2 * kp.numel(), dtype=torch.uint8).view(kp.dtype)
+    for t in ((kp, kp, ks, vs), (kp, vp, ks, ks),
+              (both[:kp.numel()].view(kp.shape), both[kp.numel() - 64:-64].view(kp.shape), ks, vs)):
+        with pytest.raises(ValueError, match="share memory"):
+            append_kv(PagedKVCache(*t), half(3, 2, 64), half(3, 2, 64), torch.zeros(3, 2, dtype=torch.int32),
+                      torch.ones(3, dtype=torch.int32))
+
+
 @pytest.mark.parametrize("kw,error,match", BAD_TABLES + [
     (dict(q=half(3, 4, 64, dtype=torch.float32)), TypeError, "float16"),
     (dict(q=half(3, 3, 64)), ValueError, "multiple of H_kv"),
@@ -188,7 +199,7 @@ def _rc(name, packed):
 NR = dict(q=256, k=512, qw=0, kw=0, cos=256, sin=256, pos=0, qo=256, ko=256, dqo=0, dko=0, dq=0, dk=0, dqw=0, dkw=0, ws=0,
           st=[64] * 14, B=1, H=4, H_kv=2, N=8, D=64, dtype=0, wdtype=0, max_pos=16, axes=1, s0=0, s1=0, s2=0, s3=0,
           pos64=0, inter=0, eps=1e-6)
-AP = dict(k=256, v=256, kp=256, vp=256, ks=256, vs=256, table=256, lens=256, offsets=0, cos=0, sin=0, pos=0, kw=0,
+AP = dict(k=256, v=256, kp=256, vp=1 << 20, ks=256, vs=1 << 20, table=256, lens=256, offsets=0, cos=0, sin=0, pos=0, kw=0,
           st=[64] * 6, eps=1e-6, T=3, B=3, width=2, pages=4, H_kv=2, P=16, D=64, dtype=0, wdtype=0, max_pos=0, axes=1,
           s0=0, s1=0, s2=0, s3=0, pos64=0, inter=0, reserved=0)
 PA = dict(q=256, kp=256, vp=256, ks=256, vs=256, table=256, lens=256, offsets=0, out=256, lse=0, ws=256, st=[64] * 5,
@@ -228,7 +239,7 @@ CACHE_CODES = [
 @pytest.mark.parametrize("kw,code", CACHE_CODES + [
     (dict(k=0), 1), (dict(cos=256), 1), (dict(cos=256, sin=256), 1), (dict(cos=256, sin=256, max_pos=4, axes=2, s1=8), 1),
     (dict(kw=256, wdtype=1), 2), (dict(kw=264), 3), (dict(v=260), 3), (dict(cos=264, sin=256, max_pos=4), 3),
-    (dict(H_kv=32768), 2)])
+    (dict(H_kv=32768), 2), (dict(vp=256), 1), (dict(vp=256 + 4 * 2 * 16 * 64 - 16), 1), (dict(vs=256 + 4), 1)])
 def test_append_c_refusals(kw, code):
     if kw.get("st", 0) is None:
         kw = dict(st=[4] + [64] * 5)
