@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
       if (key_next < key_end)
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) next_page[blk] = page_of(key_next + 16 * blk);
-      while (true) {
+      auto one_tile = [&](auto edge) {
         VBlock<D> v[2];
         float ks[2], vs[2];
 #pragma unroll
@@ -519,14 +519,13 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
         }
         vs[0] = __log2f(vs[0]);
         vs[1] = __log2f(vs[1]);
-        if (key0 + kTile > seen_by_all)
-          softmax_pv<D, NT, true>(st, s, qs, ks, vs, v, last, key0, keys, g, t, &sh_nan[warp]);
-        else
-          softmax_pv<D, NT, false>(st, s, qs, ks, vs, v, last, key0, keys, g, t, &sh_nan[warp]);
-        if (!more) break;
+        softmax_pv<D, NT, decltype(edge)::value>(st, s, qs, ks, vs, v, last, key0, keys, g, t, &sh_nan[warp]);
         key0 = key_next;
         key_next += kWarps * kTile;
-      }
+      };
+      // Two loops: the tiles that some row does not see to their end need masks and the clearing of NaN.
+      while (key0 < key_end && key0 + kTile <= seen_by_all) one_tile(std::false_type{});
+      while (key0 < key_end) one_tile(std::true_type{});
     }
 
     // ---- join the warps: m and l over the lanes of a column, then everything in shared memory
