@@ -625,23 +625,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
         const bool seen = own_last >= 0;
         const float f = seen ? (top_v / kHeadroom) / l : 0.f;
         uint16_t* out = static_cast<uint16_t*>(p.out) + token * p.out_stride[0] + head * p.out_stride[1];
-        const bool nan = *const_cast<volatile int*>(&words[kNanWord]) != 0;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
           tmem_ld_wait(o);
-          if (nan && live) {  // rare: the values that were NaN among the keys that the row sees
-            for (int key = first_hidden * kBN; key <= own_last; ++key) {
-              const int page = table[key >> p.page_shift];
-              if (page < 0 || page >= p.num_pages) continue;
-              const uint32_t* row = reinterpret_cast<const uint32_t*>(
-                  p.v_pages + (((static_cast<size_t>(page) * p.H_kv + w.h) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * D + c * 32);
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if ((nan_bytes(row[i / 4]) >> (8 * (i % 4)) & 1u) != 0) o[i] = 0x7fffffffu;
-            }
-          }
           if (live) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
@@ -657,6 +645,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
           }
         }
         if (p.lse != nullptr && live) p.lse[token * p.group * p.H_kv + head] = seen ? m_used + log2f(l) : -INFINITY;
+        if (*const_cast<volatile int*>(&words[kNanWord]) != 0 && live) {  // rare: NaN among the values that the row sees
+#pragma unroll 1
+          for (int key = first_hidden * kBN; key <= own_last; ++key) {
+            const int page = table[key >> p.page_shift];
+            if (page < 0 || page >= p.num_pages) continue;
+            const uint8_t* v = p.v_pages + (((static_cast<size_t>(page) * p.H_kv + w.h) << p.page_shift) +
+                                            (key & ((1 << p.page_shift) - 1))) * D;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 4) {
+              const uint32_t nan = nan_bytes(*reinterpret_cast<const uint32_t*>(v + d));
+              for (int i = 0; nan != 0 && i < 4; ++i)
+                if ((nan >> (8 * i) & 1u) != 0) out[d + i] = 0x7fff;  // NaN in both types
+            }
+          }
+        }
       }
     }
   }
