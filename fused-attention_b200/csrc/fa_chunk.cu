@@ -49,7 +49,7 @@ constexpr int kRegsOther = 72;
 static_assert(256 * kRegsOther + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split");
 constexpr int kSoftmaxCopy = 1;  // the softmax warpgroups' own copy of the bounded-wait loop
 // Of 16 exp2 pairs on interior tiles, those on the FMA pipe.  The conversions share that pipe's issue slots, so fewer
-// pay than in the dense forward: 3 x 1024 tokens behind 8192 keys take 290 us with one, 298 with two, 311 with four.
+// pay than in the dense forward: 3 x 1024 tokens behind 8192 keys take 294 us with one, 299 with two, 311 with four.
 constexpr int kPolyPairs = 1;
 constexpr float kHeadroom = 64.f;  // f16(448 * 64) is finite
 
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
         mbar_arrive(full + 8 * st);
       };
       // Values that some row does not see: NaN is taken out (0 * NaN is not 0) and put back at the end.  A loop of
-      // its own: inside the common one the same lines cost 8 % of the kernel.
+      // its own: the kernel then takes 294 us (289 without the clearing, 333 with it in the common loop).
       const int plain = is_k ? nmax : min(nmax, first_hidden);
       int j = 0;
       for (; ok && j < plain; ++j) convert_tile(j, std::false_type{});
