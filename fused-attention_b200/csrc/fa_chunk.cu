@@ -527,7 +527,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
           }
           *reinterpret_cast<uint4*>(tile + C::place(row, c)) = v;
         }
-        scale = p.scale_log2 * (top_k / kHeadroom) / down;
+        // Not 0, which it is for scales of zero and rounds to for tiny ones: hidden scores are -inf before they are
+        // multiplied, and -inf * 0 is NaN.  2^-126 leaves every finite score within 2^-80 of the 0 that it stands for.
+        scale = fmaxf(p.scale_log2 * (top_k / kHeadroom) / down, 0x1p-126f);
         fence_async_shared();
         mbar_arrive(BAR(BAR_Q + t));
       }

@@ -1,0 +1,80 @@
+"""Page scales of all sizes and NaN keys in attention over the paged cache, in both kernels.
+
+Bounds are those of the split kernel (tests/serving_util.py, paged64) for every key that a row sees; keys that it
+does not see have no part in them.  The chunk kernel computes some exponentials as a polynomial, off by less than 2^-13,
+in the weights and in their sum: 2^-12 beside the 2^-11 that the bound has for a weight's rounding to f16, and 2^-16 for
+the logarithms of scales that are no powers of two (an ulp of at most 126, 2^-18, twice over).  So the
+bound is taken 1.6 times there, and lse may be off by 2^-12 + 2^-14 more, in natural units."""
+import math
+
+import pytest
+import torch
+
+from tests.serving_util import half_step, half_subnormal, paged64
+from tests.test_paged_gpu import _append, _attend, _cache, _nat, batch, i32, make_cache, takes_chunk_kernel, to_gpu
+
+pytestmark = pytest.mark.gpu
+
+SPLIT = dict(lens=[300, 131], news=[3, 2], P=32, H=8, H_kv=4, D=128)
+CHUNK = dict(lens=[300, 450], news=[260, 200], P=32, H=32, H_kv=16, D=128)
+CHUNK64 = dict(lens=[700, 333], news=[300, 333], P=64, H=32, H_kv=16, D=64)
+CHUNK16 = dict(lens=[517, 260], news=[400, 260], P=16, H=40, H_kv=20, D=32)
+SHAPES = [SPLIT, CHUNK, CHUNK64, CHUNK16]
+ids = ["split", "chunk", "chunk-64", "chunk-16"]
+
+
+def is_chunk(s):
+    return takes_chunk_kernel(sum(s["news"]), len(s["lens"]), s["H"], s["H_kv"], s["D"])
+
+
+def test_shapes_take_the_kernels_they_are_named_after():
+    assert [is_chunk(s) for s in SHAPES] == [False, True, True, True]
+
+
+def check(o, lse, q, cache, table, lens, starts, scale, chunk):
+    ref, ref_lse, bound, lse_bound = paged64(q, *cache, table, lens, starts, scale)
+    if chunk:
+        bound, lse_bound = 1.6 * bound, lse_bound + math.log2(math.e) * (2.0 ** -12 + 2.0 ** -14)
+    o, lse = o.double().cpu(), lse.double().cpu()
+    assert bool(o.isfinite().all())
+    tol = half_step(q.dtype) * (ref.abs() + bound) + bound + half_subnormal(q.dtype)
+    worst = float(((o - ref).abs() / tol).max())
+    assert worst <= 1.0, worst
+    seen = ref_lse.isfinite()
+    assert bool((lse[~seen] == -math.inf).all())
+    assert bool(((lse - ref_lse).abs() <= lse_bound)[seen].all())
+
+
+def run(s, cache, q, scale=None):
+    table, starts, _ = batch(s["lens"], s["news"], s["P"])
+    scale = scale or s["D"] ** -0.5
+    o, lse = _attend(q.cuda(), _cache(*to_gpu(*cache)), table.cuda(), i32(s["lens"]), i32(starts), scale=scale, return_lse=True)
+    _nat().check_status(torch.device("cuda", torch.cuda.current_device()))
+    check(o, lse, q, cache, table, s["lens"], starts, scale, is_chunk(s))
+
+
+def queries(s, dtype, seed=5):
+    return torch.randn(sum(s["news"]), s["H"], s["D"], generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_key_scales_of_zero(s, dtype, cuda_device):
+    """Keys that stand for zero, whatever their bytes: every visible value counts alike."""
+    _, _, pages = batch(s["lens"], s["news"], s["P"])
+    kp, vp, ks, vs = make_cache(pages, s["H_kv"], s["P"], s["D"])
+    ks[:, 0] = 0
+    run(s, (kp, vp, ks, vs), queries(s, dtype))
+    run(s, (kp, vp, torch.zeros_like(ks), vs), queries(s, dtype))
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+def test_tiny_queries_and_small_key_scales(s, cuda_device):
+    """bf16 query rows of zeros and of subnormals, keys of about 2^-10, a small scale: scores next to zero."""
+    _, _, pages = batch(s["lens"], s["news"], s["P"])
+    kp, vp, ks, vs = make_cache(pages, s["H_kv"], s["P"], s["D"])
+    q = queries(s, torch.bfloat16)
+    q[::3] = 0
+    q[1::3] *= 2.0 ** -125
+    run(s, (kp, vp, torch.full_like(ks, 2.0 ** -16), vs), q)
+    run(s, (kp, vp, ks, vs), q, scale=2.0 ** -30)
