@@ -9,11 +9,13 @@
 //   * rows are (token, head of the group) pairs, so a tile of a group of G heads covers 128 / G tokens and
 //     every cached byte a block reads serves 256 rows;
 //   * K and V tiles are built by a warpgroup of their own: 16-byte pieces of a page, e4m3 -> f16 (exact),
-//     times the page's scale, into the swizzled layout that the tensor core reads.  The scale is taken
-//     relative to the sequence's largest, ref: f16(64 v8 scale / ref) is exact for power-of-two scales
-//     down to 2^-21 of the largest (below, values keep an absolute precision of 2^-40 of the largest page's
-//     magnitude; scales that are no powers of two are rounded to f16's 11 bits).  So S and O need no
-//     per-page arithmetic, and the conversions cost the softmax warps nothing;
+//     into the swizzled layout that the tensor core reads.  The tiles hold the cached values themselves;
+//   * pages' scales are float32 factors of the softmax, whatever their size.  A key's scale is part of the
+//     factor that its score has anyway.  A value's scale w rides in the weights' exponents,
+//       p' = 2^(s - m + log2 w - u),   O += p' v8,   l += 2^(u - log2 w) p',   o = 2^u O / l,
+//     with m the largest s that the row has seen and m + u the largest s + log2 w.  So P stays inside f16 and
+//     nothing that a row does not see has a part in it.  The factors are the same for kSeg keys of one page: per
+//     row and kSeg keys one exponential, two products and some ten additions and maxima more;
 //   * queries are brought to f16 by a power of two per row (exact down to 2^-31 of the row's largest
 //     element) by the thread that owns the row; P is f16.
 // Warp roles (512 threads):
@@ -44,14 +46,22 @@ constexpr int kBN = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kLaunchRegs = 128;
-constexpr int kRegsSoftmax = 184;
-constexpr int kRegsOther = 72;
+constexpr int kRegsSoftmax = 192;
+constexpr int kRegsOther = 64;
 static_assert(256 * kRegsOther + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split");
 constexpr int kSoftmaxCopy = 1;  // the softmax warpgroups' own copy of the bounded-wait loop
 // Of 16 exp2 pairs on interior tiles, those on the FMA pipe.  The conversions share that pipe's issue slots, so fewer
-// pay than in the dense forward: 3 x 1024 tokens behind 8192 keys take 294 us with one, 299 with two, 311 with four.
+// pay than in the dense forward: chunks of 1024, 437 and 1024 tokens behind up to 8192 keys take 310 us with one, 312 with
+// two; with pages of 16 keys 587 and 601 us for 4736 tokens behind 8192.
 constexpr int kPolyPairs = 1;
-constexpr float kHeadroom = 64.f;  // f16(448 * 64) is finite
+// log2 of a value's scale is taken to be at least this far below the row's best weight: then p' of a score next to m is
+// 2^-60, which f16 rounds to 0 as it would the smaller exact one, while float32 still holds what l needs of it.
+constexpr float kScaleFloor = -60.f;
+constexpr float kNoScale = -200.f;  // stands for log2 0: below every float32's
+// The softmax subtracts the rounded reference from a product that is not rounded, which is off by up to half a step of the
+// reference.  Up to here that is less than 1 and the same for all weights of a row; tiles that could hold larger scores
+// (log2 units) go through large_tile.
+constexpr float kLargeScore = 16777216.f;
 
 template <int D>
 struct ChunkCfg {
@@ -67,7 +77,8 @@ struct ChunkCfg {
   static constexpr int kOffV = kOffK + kStages * kTileBytes;
   static constexpr int kOffRaw = kOffV + kStages * kTileBytes;  // the next K and V tiles' cached bytes
   static constexpr int kOffBar = kOffRaw + 2 * 128 * D;
-  static constexpr int kSmemBytes = kOffBar + 512 + 1024;  // barriers, scan words, alignment slack
+  static constexpr int kOffFactors = kOffBar + 512;     // [softmax warp][parity of the tile][16]
+  static constexpr int kSmemBytes = kOffFactors + kSoftmaxWarps * 2 * 16 * 4 + 1024;  // alignment slack
   // Byte offset of 16-byte piece c of row r of an f16 tile (pieces of D / 8 per row).
   static __device__ __forceinline__ uint32_t place(int r, int c) {
     if constexpr (D >= 64) return (c >> 3) * kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -90,31 +101,48 @@ enum : int {
   BAR_COUNT = 28
 };
 
-// One 16-byte piece of a cached row -> 16 f16 values times f, or times f 2^-14 where `small`: the first product is
-// exact (a byte's value is a multiple of 2^-9), so there is one rounding either way.
-constexpr float kSmall = 1.f / 16384;  // f16's smallest normal number: a smaller factor would lose bits itself
-template <bool small>
-__device__ __forceinline__ void dequant16(const uint4& raw, uint32_t f, uint4& lo, uint4& hi) {
+// One 16-byte piece of a cached row -> 16 f16 values.
+__device__ __forceinline__ void to_f16(const uint4& raw, uint4& lo, uint4& hi) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   uint32_t h[8];
-  const __half2 scale = *reinterpret_cast<const __half2*>(&f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t a, b;
+  for (int i = 0; i < 4; ++i)
     asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
-        : "=r"(a), "=r"(b) : "r"(w[i]));
-    __half2 ha = *reinterpret_cast<const __half2*>(&a), hb = *reinterpret_cast<const __half2*>(&b);
-    if constexpr (small) {
-      ha = __hmul2(ha, __float2half2_rn(kSmall));
-      hb = __hmul2(hb, __float2half2_rn(kSmall));
-    }
-    ha = __hmul2(ha, scale);
-    hb = __hmul2(hb, scale);
-    h[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
-    h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
-  }
+        : "=r"(h[2 * i]), "=r"(h[2 * i + 1]) : "r"(w[i]));
   lo = make_uint4(h[0], h[1], h[2], h[3]);
   hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// The largest of N scores from `r` on.
+template <int N>
+__device__ __forceinline__ float top_of(const uint32_t* r) {
+  constexpr int kChains = N / 8;
+  float top[kChains];
+#pragma unroll
+  for (int u = 0; u < kChains; ++u) top[u] = fmaxf(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1]));
+#pragma unroll
+  for (int i = kChains; i < N / 2; ++i)
+    top[i % kChains] = fmax3(top[i % kChains], __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+  if constexpr (kChains == 4) return fmaxf(fmax3(top[0], top[1], top[2]), top[3]);
+  return fmaxf(top[0], top[1]);
+}
+
+// Weights p' = 2^(s factor + shift) of N scores as pairs of f16, added up in `sum`; the first pair is number kFirst of
+// its 16.  kPolyPairs of those are a polynomial where `poly` (not on tiles with hidden keys, whose scores are -inf).
+template <int N, int kFirst, bool poly>
+__device__ __forceinline__ void weigh(const uint32_t* r, float factor, float shift, uint64_t (&sum)[4], uint32_t* pk) {
+  const uint64_t factor2 = f2(factor, factor), shift2 = f2(shift, shift);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const uint64_t x2 = ffma2(f2u(r[2 * i], r[2 * i + 1]), factor2, shift2);
+    uint64_t p2;
+    if (poly && (kFirst + i) % (16 / kPolyPairs) == 16 / kPolyPairs - 1)
+      p2 = exp2_poly2(x2);
+    else
+      p2 = f2(ex2_approx(f2lo(x2)), ex2_approx(f2hi(x2)));
+    sum[i & 3] = fadd2(sum[i & 3], p2);
+    pk[i] = pack2<false>(f2lo(p2), f2hi(p2));
+  }
 }
 
 // S = Q K^T for one tile.
@@ -210,7 +238,65 @@ __device__ __forceinline__ ChunkWork find_work(const PagedParams& p, int* words)
   return {words[0], words[1], words[2], words[3], words[4], words[5]};
 }
 
-template <int D>
+// One tile of a row's softmax with scores of any size, which are rounded before the reference is subtracted: the
+// same sums as in the kernel's loop, through TMEM in pieces of 32 columns.  factors: the segments' key scales, then
+// log2 of their value scales; keys from `hidden` on are not seen.
+template <int D, int kSeg>
+__device__ __noinline__ void large_tile(uint32_t t_s, uint32_t t_o, const float* factors, float row_factor, int hidden,
+                                        bool first, float& m, float& u, float& l) {
+  constexpr int kSegs = kBN / kSeg, kPiece = kSeg < 32 ? kSeg : 32;
+  uint32_t x[32];
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kBN / 32; ++c) {
+    tmem_ld32(t_s + c * 32, x);
+    tmem_ld_wait(x);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float v = __fmul_rn(__uint_as_float(x[i]), factors[(c * 32 + i) / kSeg] * row_factor);
+      x[i] = __float_as_uint(c * 32 + i < hidden ? v : -INFINITY);
+    }
+    top = fmaxf(top, top_of<32>(x));
+    tmem_st32(t_s + c * 32, x);
+  }
+  tmem_st_wait();
+  const bool up = top > m + kRescaleThreshold;
+  const float m_new = up ? top : m, u_old = up ? u + (m - m_new) : u;
+  float top_u = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kBN / 32; ++c) {
+    tmem_ld32(t_s + c * 32, x);
+    tmem_ld_wait(x);
+#pragma unroll
+    for (int i = 0; i < 32; i += kPiece)
+      top_u = fmaxf(top_u, (top_of<kPiece>(&x[i]) - m_new) + factors[kSegs + (c * 32 + i) / kSeg]);
+  }
+  const bool up_u = top_u > u_old + kRescaleThreshold;
+  const float u_new = up_u ? top_u : u_old;
+  if (!first && __any_sync(0xffffffffu, up_u)) rescale_o<D>(t_o, up_u ? ex2_approx(u_old - u_new) : 1.f);
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < kBN / 32; ++c) {
+    tmem_ld32(t_s + c * 32, x);
+    tmem_ld_wait(x);
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float log_scale = fmaxf(factors[kSegs + (c * 32 + i) / kSeg], u_new + kScaleFloor) - u_new;
+      const float a = ex2_approx(__fsub_rn(__uint_as_float(x[i]), m_new) + log_scale);
+      const float b = ex2_approx(__fsub_rn(__uint_as_float(x[i + 1]), m_new) + log_scale);
+      sum = fmaf(a + b, ex2_approx(-log_scale), sum);
+      pk[i / 2] = pack2<false>(a, b);
+    }
+    tmem_st16(t_s + c * 16, pk);  // over columns that have been read
+  }
+  l = l * (up ? ex2_approx(m - m_new) : 1.f) + sum;
+  m = m_new;
+  u = u_new;
+}
+
+// kSeg: keys that share their factors for sure, the page size up to 64.
+template <int D, int kSeg>
 __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedParams p) {
   using C = ChunkCfg<D>;
   constexpr int ST = C::kStages;
@@ -221,7 +307,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kOffBar + 8 * BAR_COUNT);
   int* words = reinterpret_cast<int*>(smem + C::kOffBar + 8 * BAR_COUNT + 16);
-  float* maxima = reinterpret_cast<float*>(smem + C::kOffBar + 8 * BAR_COUNT + 48);  // [2][16]
   const uint32_t bar0 = smem_u32(bars);
 #define BAR(i) (bar0 + 8u * static_cast<uint32_t>(i))
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -251,29 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
     return;
   }
 
-  // The largest page scales of the keys that the block reads.
-  float top_k = 0.f, top_v = 0.f;
   const int pages = ((keys - 1) >> p.page_shift) + 1;
-  for (int i = threadIdx.x; i < pages; i += kThreads) {
-    const int page = table[i];
-    if (page < 0 || page >= p.num_pages) {
-      record_error(p.status, kDevBadIndex, w.b);
-    } else {
-      const size_t at = static_cast<size_t>(page) * p.H_kv + w.h;
-      const float k = p.k_scales[at], v = p.v_scales[at];
-      if (k < INFINITY) top_k = fmaxf(top_k, k);
-      if (v < INFINITY) top_v = fmaxf(top_v, v);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    top_k = fmaxf(top_k, __shfl_xor_sync(0xffffffffu, top_k, o));
-    top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
-  }
-  if (lane == 0) {
-    maxima[warp] = top_k;
-    maxima[16 + warp] = top_v;
-  }
   if (threadIdx.x == 0) {
     mbar_init(BAR(BAR_Q), 128);
     mbar_init(BAR(BAR_Q + 1), 128);
@@ -380,7 +443,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       constexpr int kMost = 3;                   // blocks of a warp, at most
       const int row_in_block = lane / kLanes, piece = lane % kLanes;
       const uint8_t* bytes = (is_k ? p.k_pages : p.v_pages) + piece * 16;
-      const float* scales = is_k ? p.k_scales : p.v_scales;
       uint8_t* ring = smem + (is_k ? C::kOffK : C::kOffV);
       // A block's bytes wait in shared memory (asynchronous copies, each thread its own pieces) from the
       // moment the block of the tile before has been converted: nearly a tile's time in flight.
@@ -388,11 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       const uint32_t full = BAR(is_k ? BAR_KFULL : BAR_VFULL), empty = BAR(is_k ? BAR_KEMPTY : BAR_VEMPTY);
       const uint32_t page_bytes = static_cast<uint32_t>(D) << p.page_shift;
       const int page_mask = (1 << p.page_shift) - 1;
-      float top = 0.f;
-      for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, maxima[(is_k ? 0 : 16) + i]);
-      const float inv = top > 0.f ? kHeadroom / top : 0.f;
-      int page[kMost] = {};     // of the block's next copy, read a tile ahead
-      float scale[kMost] = {};  // of the bytes that wait
+      int page[kMost] = {};  // of the block's next copy, read a tile ahead
       auto page_of = [&](int j, int blk) {
         return table[min((j * kBN + (first_block + blk) * 16) >> p.page_shift, pages - 1)];
       };
@@ -406,7 +464,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
           for (int i = 0; i < kLoads; ++i)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(raw + blk * 16 * D + i * 512)),
                          "l"(src + i * 512) : "memory");
-          scale[blk] = scales[at];
           page[blk] = page_of(j + 1, blk);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -429,35 +486,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
               asm volatile("cp.async.wait_group 1;" ::: "memory");
             else
               asm volatile("cp.async.wait_group 2;" ::: "memory");
-            const float relative = scale[blk] * inv;
-            const bool small = relative < kSmall;
-            const __half2 f2h = __float2half2_rn(small ? relative * (1.f / kSmall) : relative);
-            const uint32_t factor = *reinterpret_cast<const uint32_t*>(&f2h);
             const int row0 = (first_block + blk) * 16 + row_in_block;
-            auto convert = [&](auto is_small) {
 #pragma unroll
-              for (int i = 0; i < kLoads; ++i) {
-                const int row = row0 + i * kRowsPerLoad;
-                uint4 v = *reinterpret_cast<const uint4*>(raw + blk * 16 * D + i * 512);
-                if (j * kBN + row >= keys) v = make_uint4(0, 0, 0, 0);  // behind the last key
-                if constexpr (decltype(clean)::value) {
-                  const uint4 nan = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
-                  if ((nan.x | nan.y | nan.z | nan.w) != 0) *const_cast<volatile int*>(&words[kNanWord]) = 1;
-                  v = make_uint4(v.x & ~nan.x, v.y & ~nan.y, v.z & ~nan.z, v.w & ~nan.w);
-                }
-                uint4 lo, hi;
-                dequant16<decltype(is_small)::value>(v, factor, lo, hi);
-                // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes
-                // of a row then meet all banks
-                const bool swap = D == 128 && piece >= 4;
-                *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 1 : 0))) = swap ? hi : lo;
-                *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 0 : 1))) = swap ? lo : hi;
+            for (int i = 0; i < kLoads; ++i) {
+              const int row = row0 + i * kRowsPerLoad;
+              uint4 v = *reinterpret_cast<const uint4*>(raw + blk * 16 * D + i * 512);
+              if (j * kBN + row >= keys) v = make_uint4(0, 0, 0, 0);  // behind the last key
+              if constexpr (decltype(clean)::value) {
+                const uint4 nan = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
+                if ((nan.x | nan.y | nan.z | nan.w) != 0) *const_cast<volatile int*>(&words[kNanWord]) = 1;
+                v = make_uint4(v.x & ~nan.x, v.y & ~nan.y, v.z & ~nan.z, v.w & ~nan.w);
               }
-            };
-            if (small)
-              convert(std::true_type{});
-            else
-              convert(std::false_type{});
+              uint4 lo, hi;
+              to_f16(v, lo, hi);
+              // lanes of the two halves of a row store their two pieces in opposite order: the eight lanes
+              // of a row then meet all banks
+              const bool swap = D == 128 && piece >= 4;
+              *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 1 : 0))) = swap ? hi : lo;
+              *reinterpret_cast<uint4*>(tile + C::place(row, 2 * piece + (swap ? 0 : 1))) = swap ? lo : hi;
+            }
             copy(j + 1, blk);
           }
         }
@@ -465,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
         mbar_arrive(full + 8 * st);
       };
       // Values that some row does not see: NaN is taken out (0 * NaN is not 0) and put back at the end.  A loop of
-      // its own: the kernel then takes 294 us (289 without the clearing, 333 with it in the common loop).
+      // its own: it costs 2 % of the kernel's time, in the common loop it cost 15 %.
       const int plain = is_k ? nmax : min(nmax, first_hidden);
       int j = 0;
       for (; ok && j < plain; ++j) convert_tile(j, std::false_type{});
@@ -489,13 +536,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       const int own_last = live ? w.before + r / p.group : 0;
       const int last = max(0, own_last);
       const int full = max(0, w.before + (w.r0 + t * kBM) / p.group);  // every row of the tile sees keys <= full
-      top_k = top_v = 0.f;
-      for (int i = 0; i < kThreads / 32; ++i) {
-        top_k = fmaxf(top_k, maxima[i]);
-        top_v = fmaxf(top_v, maxima[16 + i]);
+      // The tile's factors: lane g loads the key scale of segment g, lane kSegs + g the value scale, a tile ahead
+      // (and the page two ahead); the warp's lanes then read them in shared memory.
+      constexpr int kSegs = kBN / kSeg;
+      float* factors = reinterpret_cast<float*>(smem + C::kOffFactors) + warp * 32;
+      const bool loads = lane < 2 * kSegs;
+      const float* scales = lane < kSegs ? p.k_scales : p.v_scales;
+      auto page_of = [&](int j) { return table[min((j * kBN + lane % kSegs * kSeg) >> p.page_shift, pages - 1)]; };
+      auto scale_of = [&](int page) {
+        if (page < 0 || page >= p.num_pages) {
+          record_error(p.status, kDevBadIndex, w.b);
+          page = 0;
+        }
+        return scales[static_cast<size_t>(page) * p.H_kv + w.h];
+      };
+      float next = 0.f;
+      int next_page = 0;
+      if (loads) {
+        next = scale_of(page_of(0));
+        next_page = page_of(1);
       }
       // Q row -> f16 by a power of two
-      float scale;
+      float row_factor, large_scale;  // a key scale from which the warp's scores could be large
       {
         uint8_t* tile = smem + C::kOffQ + t * C::kTileBytes;
         const uint16_t* q = static_cast<const uint16_t*>(p.q) + token * p.q_stride[0] + head * p.q_stride[1];
@@ -527,9 +589,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
           }
           *reinterpret_cast<uint4*>(tile + C::place(row, c)) = v;
         }
-        // Not 0, which it is for scales of zero and rounds to for tiny ones: hidden scores are -inf before they are
-        // multiplied, and -inf * 0 is NaN.  2^-126 leaves every finite score within 2^-80 of the 0 that it stands for.
-        scale = fmaxf(p.scale_log2 * (top_k / kHeadroom) / down, 0x1p-126f);
+        row_factor = p.scale_log2 / down;
+        float size = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&x[c][i]));
+            size += fabsf(v.x) + fabsf(v.y);
+          }
+        size *= row_factor;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
+        large_scale = kLargeScore / (448.f * size);
         fence_async_shared();
         mbar_arrive(BAR(BAR_Q + t));
       }
@@ -537,22 +609,97 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
       const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
       const uint32_t tS = tmem + t * 128 + lane_off;
       const uint32_t tO = tmem + 256 + t * 128 + lane_off;
-      float m_used = -INFINITY;
+      // References: m of the scores, m + u of the scores plus log2 of their value's scale (u by itself, small next to m).
+      float m = -INFINITY, u = 0.f;
       float l = 0.f;
       bool ok = true;
       for (int j = 0; j < nkv; ++j) {
+        float* tile_factors = factors + (j & 1) * 16;
+        const bool large = __any_sync(0xffffffffu, lane < kSegs && next > large_scale);
+        if (loads) {
+          tile_factors[lane] = lane < kSegs ? next : (next > 0.f ? log2f(next) : kNoScale);
+          next = scale_of(next_page);
+          next_page = page_of(j + 2);
+        }
+        __syncwarp();
         if (!(ok = warp_all(mbar_wait<kSoftmaxCopy>(BAR(BAR_SFULL + t), j & 1, p.status, kDevTimeoutS)))) break;
         tc_fence_after();
+        const int kbase = j * kBN;
+        if (large) {
+          large_tile<D, kSeg>(tS, tO, tile_factors, row_factor, last + 1 - kbase, j == 0, m, u, l);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(BAR(BAR_PFULLA + t));
+          mbar_arrive(BAR(BAR_PFULLB + t));
+          continue;
+        }
         uint32_t s[NCH][32];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) tmem_ld32(tS + c * 32, s[c]);
 #pragma unroll
         for (int c = 0; c < NCH; ++c) tmem_ld_wait(s[c]);
-        const int kbase = j * kBN;
         const bool masked = kbase + kBN - 1 > full;
-        const uint64_t scale2 = f2(scale, scale);
-        uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
-        float alpha = 1.f;
+        // On tiles with hidden keys not 0, which it is for a scale of zero and rounds to for tiny ones: hidden scores are
+        // -inf before they are multiplied, and -inf * 0 is NaN.  2^-126 leaves every finite score within 2^-80 of the 0
+        // that it stands for.
+        auto score_factor = [&](int g, auto hides) {
+          const float f = tile_factors[g] * row_factor;
+          return decltype(hides)::value ? fmaxf(f, 0x1p-126f) : f;
+        };
+        uint64_t sum2 = 0ull;
+        // The weights of half a tile, into TMEM and sum2.  hides: the tile has hidden keys, no polynomial.
+        auto weigh_half = [&](int h, auto hides) {
+          constexpr bool poly = !decltype(hides)::value;
+          constexpr int kPiece = kSeg < 32 ? kSeg : 32;
+          float factor, shift, log_scale;
+          uint64_t sum[4];
+#pragma unroll
+          for (int c = h * NCH / 2; c < (h + 1) * NCH / 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int at = 0; at < 32; at += kPiece) {
+              const int col = c * 32 + at, g = col / kSeg;
+              if (col % kSeg == 0) {
+                factor = score_factor(g, hides);
+                log_scale = fmaxf(tile_factors[kSegs + g], u + kScaleFloor) - u;
+                shift = log_scale - m;
+                sum[0] = sum[1] = sum[2] = sum[3] = 0ull;
+              }
+              if (at == 0)
+                weigh<kPiece, 0, poly>(&s[c][0], factor, shift, sum, pk);
+              else
+                weigh<kPiece, kPiece % 32 / 2, poly>(&s[c][kPiece % 32], factor, shift, sum, pk + kPiece % 32 / 2);
+              if ((col + kPiece) % kSeg == 0) {
+                const float back = ex2_approx(-log_scale);
+                sum2 = ffma2(fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3])), f2(back, back), sum2);
+              }
+            }
+            tmem_st16(tS + c * 16, pk);
+          }
+        };
+        // Raises the references where the tile's maxima pass one by the threshold; l's and O's factors for that.
+        float alpha = 1.f, alpha_o = 1.f;
+        auto raise = [&](auto hides) {
+          float top = -INFINITY, top_w = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < kSegs; ++g) {
+            float x = top_of<kSeg < 32 ? kSeg : 32>(&s[g * kSeg / 32][g * kSeg % 32]);
+            if constexpr (kSeg == 64) x = fmaxf(x, top_of<32>(s[2 * g + 1]));
+            x *= score_factor(g, hides);
+            top = fmaxf(top, x);
+            top_w = fmaxf(top_w, x + tile_factors[kSegs + g]);
+          }
+          const float mw = m + u;
+          const bool up = top > m + kRescaleThreshold || top_w > mw + kRescaleThreshold;
+          if (up) {
+            const float m_new = fmaxf(m, top), u_new = fmaxf(mw, top_w) - m_new;
+            alpha = ex2_approx(m - m_new);
+            alpha_o = ex2_approx((m - m_new) + (u - u_new));
+            m = m_new;
+            u = u_new;
+          }
+          return __any_sync(0xffffffffu, up) != 0;
+        };
         if (masked || j == 0) {
           if (masked) {
 #pragma unroll
@@ -561,71 +708,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
               for (int i = 0; i < 32; ++i)
                 if (kbase + c * 32 + i > last) s[c][i] = __float_as_uint(-INFINITY);
           }
-          const float mt = row_max<NCH>(s) * scale;
-          const bool upd = mt > m_used + kRescaleThreshold;
-          const float m_new = upd ? mt : m_used;
-          alpha = ex2_approx(m_used - m_new);
-          const uint64_t negm2 = f2(-m_new, -m_new);
-#pragma unroll
-          for (int c = 0; c < NCH; ++c) {
-            uint32_t pk[16];
-            softmax_chunk<false, 0>(s[c], scale2, negm2, sum2, pk);
-            tmem_st16(tS + c * 16, pk);
-          }
-          if (j > 0 && __any_sync(0xffffffffu, upd)) rescale_o<D>(tO, alpha);
-          m_used = m_new;
+          const bool any = raise(std::true_type{});
+          if (j > 0 && any) rescale_o<D>(tO, alpha_o);
+          weigh_half(0, std::true_type{});
+          weigh_half(1, std::true_type{});
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(BAR(BAR_PFULLA + t));
           mbar_arrive(BAR(BAR_PFULLB + t));
         } else {
-          // the first half with the running reference while the row's new maximum is computed beside it
-          uint64_t negm2 = f2(-m_used, -m_used);
-#pragma unroll
-          for (int c = 0; c < NCH / 2; ++c) {
-            uint32_t pk[16];
-            softmax_chunk<false, kPolyPairs>(s[c], scale2, negm2, sum2, pk);
-            tmem_st16(tS + c * 16, pk);
-          }
-          const float mt = row_max<NCH>(s) * scale;
-          const bool upd = mt > m_used + kRescaleThreshold;
-          if (__any_sync(0xffffffffu, upd)) {
-            const float m_new = upd ? mt : m_used;
-            alpha = ex2_approx(m_used - m_new);
-            negm2 = f2(-m_new, -m_new);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) sum2[u] = 0ull;
-#pragma unroll
-            for (int c = 0; c < NCH / 2; ++c) {
-              uint32_t pk[16];
-              softmax_chunk<false, 0>(s[c], scale2, negm2, sum2, pk);
-              tmem_st16(tS + c * 16, pk);
-            }
-            rescale_o<D>(tO, alpha);
-            m_used = m_new;
+          // the first half with the running references while the tile's maxima are computed beside it
+          weigh_half(0, std::false_type{});
+          if (raise(std::false_type{})) {
+            sum2 = 0ull;
+            weigh_half(0, std::false_type{});
+            rescale_o<D>(tO, alpha_o);
           }
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(BAR(BAR_PFULLA + t));
-#pragma unroll
-          for (int c = NCH / 2; c < NCH; ++c) {
-            uint32_t pk[16];
-            softmax_chunk<false, kPolyPairs>(s[c], scale2, negm2, sum2, pk);
-            tmem_st16(tS + c * 16, pk);
-          }
+          weigh_half(1, std::false_type{});
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(BAR(BAR_PFULLB + t));
         }
-        const uint64_t s01 = fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3]));
-        l = l * alpha + (f2lo(s01) + f2hi(s01));
+        l = l * alpha + (f2lo(sum2) + f2hi(sum2));
       }
       if (ok) ok = mbar_wait<kSoftmaxCopy>(BAR(BAR_OFULL + t), 0, p.status, kDevTimeoutO);
       ok = warp_all(ok);
       if (ok) {
         tc_fence_after();
         const bool seen = own_last >= 0;
-        const float f = seen ? (top_v / kHeadroom) / l : 0.f;
+        const float f = seen ? exp2f(u) / l : 0.f;
         uint16_t* out = static_cast<uint16_t*>(p.out) + token * p.out_stride[0] + head * p.out_stride[1];
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -646,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
             }
           }
         }
-        if (p.lse != nullptr && live) p.lse[token * p.group * p.H_kv + head] = seen ? m_used + log2f(l) : -INFINITY;
+        if (p.lse != nullptr && live) p.lse[token * p.group * p.H_kv + head] = seen ? m + log2f(l) : -INFINITY;
         if (*const_cast<volatile int*>(&words[kNanWord]) != 0 && live) {  // rare: NaN among the values that the row sees
 #pragma unroll 1
           for (int key = first_hidden * kBN; key <= own_last; ++key) {
@@ -675,12 +789,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
   }
 }
 
-template <int D>
+template <int D, int kSeg>
 cudaError_t launch_chunk_t(const PagedParams& p, int blocks, cudaStream_t stream) {
   static std::atomic<bool> smem_set[64];
-  const cudaError_t e = opt_in_smem(paged_chunk_kernel<D>, ChunkCfg<D>::kSmemBytes, smem_set, kLaunchRegs);
+  const cudaError_t e = opt_in_smem(paged_chunk_kernel<D, kSeg>, ChunkCfg<D>::kSmemBytes, smem_set, kLaunchRegs);
   if (e != cudaSuccess) return e;
-  paged_chunk_kernel<D><<<blocks, kThreads, ChunkCfg<D>::kSmemBytes, stream>>>(p);
+  paged_chunk_kernel<D, kSeg><<<blocks, kThreads, ChunkCfg<D>::kSmemBytes, stream>>>(p);
   return cudaGetLastError();
 }
 
@@ -691,11 +805,13 @@ static long long chunk_blocks(const PagedParams& p) {
   return (static_cast<long long>(p.T) * p.group / (2 * kBM) + p.B) * p.H_kv;
 }
 
-// Which kernel takes a call, by the two's times for its 128-key tiles.  The split kernel spends c1 = 7 ns of
-// the whole GPU on 16 rows and 128 keys at D = 128 (4.2 ns at D = 64), the chunk kernel c2 = 2.25 us (1.6 us)
-// of one SM on 256 rows, filled or not: c2 / c1 is about 320 at D = 128 and 400 below.  Measured at D = 128,
-// 8 K/V heads, groups of 4, 8192 keys, chunk / split: 16 x 16 tokens 152 / 244 us, 1 x 256 tokens 167 / 215,
-// 4 x 16 tokens 144 / 78, 1 x 64 tokens 165 / 74.  Only averages are known here: sequences' lengths are on the device.
+// Which kernel takes a call, by the two's times for its 128-key tiles.  The split kernel spends c1 = 7 ns of the whole GPU
+// on 16 rows and 128 keys at D = 128 (4.2 ns at D = 64), the chunk kernel c2 of one SM on a block's rows: 2.2 us
+// with up to 128 of them, 2.6 to 2.8 with more.  The border is c2 / c1 = 320 at D = 128 and 400 below.  Measured at
+// D = 128, 8 K/V heads, groups of 4, 8192 keys, chunk / split in us: 16 x 16 tokens 151 / 235, 16 x 10 tokens 148 / 183,
+// 1 x 256 tokens 170 / 200, 1 x 208 tokens 171 / 169, 1 x 160 tokens (the border) 170 / 135, 4 x 16 tokens 144 / 71, 1 x 64
+// tokens 170 / 67: with one sequence the border is low, with many it is not.  Only averages are known here:
+// sequences' lengths are on the device.
 bool use_chunk(const PagedParams& p, int D) {
   if (chunk_blocks(p) > 0x7fffffffLL) return false;
 #ifdef FA_CHUNK_ROWS  // a build that picks by rows alone, to time one kernel against the other
@@ -710,9 +826,14 @@ bool use_chunk(const PagedParams& p, int D) {
 
 cudaError_t launch_chunk(const PagedParams& p, int D, cudaStream_t stream) {
   const int blocks = static_cast<int>(chunk_blocks(p));
-  if (D == 32) return launch_chunk_t<32>(p, blocks, stream);
-  if (D == 64) return launch_chunk_t<64>(p, blocks, stream);
-  if (D == 128) return launch_chunk_t<128>(p, blocks, stream);
+#define FA_CHUNK_CASE(DD) \
+  if (D == DD)                                                                                                  \
+    return p.page_shift == 4 ? launch_chunk_t<DD, 16>(p, blocks, stream)                                        \
+                             : (p.page_shift == 5 ? launch_chunk_t<DD, 32>(p, blocks, stream) : launch_chunk_t<DD, 64>(p, blocks, stream));
+  FA_CHUNK_CASE(32)
+  FA_CHUNK_CASE(64)
+  FA_CHUNK_CASE(128)
+#undef FA_CHUNK_CASE
   return cudaErrorInvalidValue;
 }
 

@@ -78,3 +78,81 @@ def test_tiny_queries_and_small_key_scales(s, cuda_device):
     q[1::3] *= 2.0 ** -125
     run(s, (kp, vp, torch.full_like(ks, 2.0 ** -16), vs), q)
     run(s, (kp, vp, ks, vs), q, scale=2.0 ** -30)
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+@pytest.mark.parametrize("zero", ["keys", "values", "both"])
+def test_zero_tokens(s, zero, cuda_device):
+    """Appended zeros, of one head or of all: their pages have the smallest scale there is, 2^-126."""
+    table, starts, pages = batch(s["lens"], s["news"], s["P"])
+    for heads in (slice(0, 1), slice(None)):
+        cache = _cache(*to_gpu(*make_cache(pages, s["H_kv"], s["P"], s["D"], junk=True)))
+        all_starts = [0]
+        for L in s["lens"]:
+            all_starts.append(all_starts[-1] + L)
+        x = torch.randn(all_starts[-1], 2, s["H_kv"], s["D"], generator=torch.Generator().manual_seed(3)).half()
+        if zero != "values":
+            x[:, 0, heads] = 0
+        if zero != "keys":
+            x[:, 1, heads] = 0
+        xg = x.cuda()
+        _append(cache, xg[:, 0], xg[:, 1], table.cuda(), i32(s["lens"]), i32(all_starts))
+        tensors = [t.view(torch.uint8).cpu().view(t.dtype) if t.element_size() == 1 else t.cpu()
+                   for t in (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales)]
+        assert float((tensors[2] if zero != "values" else tensors[3])[int(table[0, 0]), 0]) == 2.0 ** -126
+        run(s, tensors, queries(s, torch.float16))
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+@pytest.mark.parametrize("power", [30, 60, 100])
+@pytest.mark.parametrize("which", ["keys", "values"])
+def test_large_tokens_that_a_row_does_not_see(s, power, which, cuda_device):
+    """The page of the last tokens is 2^power above the others (a bf16 outlier): the rows before them are as exact
+    as without it, and so are those of pages far below, where the scores pick them."""
+    table, _, pages = batch(s["lens"], s["news"], s["P"])
+    kp, vp, ks, vs = make_cache(pages, s["H_kv"], s["P"], s["D"])
+    for b, L in enumerate(s["lens"]):
+        (ks if which == "keys" else vs)[int(table[b, (L - 1) // s["P"]])] *= 2.0 ** power
+        if which == "values":
+            vs[int(table[b, 1])] *= 2.0 ** -power
+    run(s, (kp, vp, ks, vs), queries(s, torch.bfloat16) * 3)
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_scales_that_are_no_powers_of_two(s, dtype, cuda_device):
+    """Any finite scale is used as it is, in float32: large scores (20 and more) keep their weights."""
+    _, _, pages = batch(s["lens"], s["news"], s["P"])
+    kp, vp, ks, vs = make_cache(pages, s["H_kv"], s["P"], s["D"])
+    g = torch.Generator().manual_seed(8)
+    ks = 2.0 ** -7 * (0.5 + torch.rand(ks.shape, generator=g))
+    vs = vs * (0.5 + torch.rand(vs.shape, generator=g))
+    run(s, (kp, vp, ks, vs), (queries(s, torch.float32) * 8).to(dtype))
+
+
+def test_single_tokens_and_a_chunk_in_one_batch(cuda_device):
+    """A serving batch: 31 sequences that decode and one prompt's chunk, lengths from 1 to 1500."""
+    g = torch.Generator().manual_seed(2)
+    lens = [1 + int(x) for x in torch.randint(0, 1500, (32,), generator=g)]
+    news = [1] * 32
+    lens[17], news[17], lens[3] = 1400, 512, 1
+    s = dict(lens=lens, news=news, P=64, H=32, H_kv=8, D=128)
+    _, _, pages = batch(lens, news, 64)
+    assert is_chunk(s)
+    run(s, make_cache(pages, 8, 64, 128), queries(s, torch.bfloat16))
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+def test_bad_pages_are_reported(s, cuda_device):
+    """A page out of range, first and last of a sequence: code 111, and the next call works."""
+    nat = _nat()
+    table, starts, pages = batch(s["lens"], s["news"], s["P"])
+    cache = make_cache(pages, s["H_kv"], s["P"], s["D"])
+    gpu, q = _cache(*to_gpu(*cache)), queries(s, torch.float16).cuda()
+    for at, page in ((0, pages), (0, -1), ((s["lens"][0] - 1) // s["P"], 1 << 30)):
+        bad = table.clone()
+        bad[0, at] = page
+        _attend(q, gpu, bad.cuda(), i32(s["lens"]), i32(starts))
+        with pytest.raises(nat.KernelError, match="outside its table"):
+            nat.check_status(cuda_device)
+    run(s, cache, queries(s, torch.float16))
