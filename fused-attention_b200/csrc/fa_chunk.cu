@@ -136,11 +136,14 @@ __device__ __forceinline__ void weigh(const uint32_t* r, float factor, float shi
   for (int i = 0; i < N / 2; ++i) {
     const uint64_t x2 = ffma2(f2u(r[2 * i], r[2 * i + 1]), factor2, shift2);
     uint64_t p2;
-    if (poly && (kFirst + i) % (16 / kPolyPairs) == 16 / kPolyPairs - 1)
+    if (poly && (kFirst + i) % (16 / kPolyPairs) == 16 / kPolyPairs - 1) {
+      // the polynomial is finite whatever x is: NaN reaches the row through the sum
       p2 = exp2_poly2(x2);
-    else
+      sum[i & 3] = fadd2(sum[i & 3], ffma2(x2, 0ull, p2));
+    } else {
       p2 = f2(ex2_approx(f2lo(x2)), ex2_approx(f2hi(x2)));
-    sum[i & 3] = fadd2(sum[i & 3], p2);
+      sum[i & 3] = fadd2(sum[i & 3], p2);
+    }
     pk[i] = pack2<false>(f2lo(p2), f2hi(p2));
   }
 }

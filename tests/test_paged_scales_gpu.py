@@ -156,3 +156,29 @@ def test_bad_pages_are_reported(s, cuda_device):
         with pytest.raises(nat.KernelError, match="outside its table"):
             nat.check_status(cuda_device)
     run(s, cache, queries(s, torch.float16))
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+def test_nan_keys_of_every_place_in_a_tile(s, cuda_device):
+    """A NaN in a cached key makes NaN of the rows that see it, wherever in a tile of 32 or 128 keys it stands, and
+    changes no other row."""
+    table, starts, pages = batch(s["lens"], s["news"], s["P"])
+    kp, vp, ks, vs = make_cache(pages, s["H_kv"], s["P"], s["D"])
+    q = queries(s, torch.float16)
+    args = (table.cuda(), i32(s["lens"]), i32(starts))
+    ref = _attend(q.cuda(), _cache(*to_gpu(kp, vp, ks, vs)), *args).cpu()
+    group = s["H"] // s["H_kv"]
+    for key0 in (0, 128):
+        for shift in range(0, 128, s["H_kv"]):  # another key for each head but the last
+            bad = kp.clone()
+            expected = torch.zeros(ref.shape[:2], dtype=torch.bool)
+            for h in range(s["H_kv"] - 1):
+                key = key0 + (shift + h) % 128
+                bad.view(torch.uint8)[int(table[0, key // s["P"]]), h, key % s["P"], (7 * h) % s["D"]] = 0x7f | (h % 2 << 7)
+                first = max(0, key - (s["lens"][0] - s["news"][0]))  # the first token that sees it
+                expected[first:starts[1], h * group:(h + 1) * group] = True
+            o, lse = _attend(q.cuda(), _cache(*to_gpu(bad, vp, ks, vs)), *args, return_lse=True)
+            o = o.cpu()
+            assert bool(o[expected].isnan().all()) and torch.equal(lse.cpu().isnan(), expected)
+            assert torch.equal(o[~expected], ref[~expected])
+    _nat().check_status(cuda_device)
