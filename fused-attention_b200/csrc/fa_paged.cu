@@ -26,10 +26,11 @@
 //     spare the conversions, but it is not a machine instruction here (it expands into conversions and
 //     f16 products; measured 74 us instead of 68 for 32 sequences of up to 8192).
 //   * Types.  e4m3 is exact in f16, so K and V lose nothing; bf16 queries are brought into f16's
-//     range by a power of two per row (exact).  P is f16 relative to a reference of s +
-//     log2(v_scale), so the pages' scales ride in P's exponent and a page with a small scale loses no
-//     precision; the softmax sum has its own reference, per thread, in float32.  A reference moves
-//     only when a score passes it by 2^kSlack: O is rescaled, and lanes compare notes, only then.
+//     range by a power of two per row (exact).  A row has two references, float32: m of its scores, which
+//     its sum l is relative to, and u of s - m + log2(v_scale).  P is f16, 2^(s - m + log2(v_scale) - u), so
+//     the pages' scales ride in P's exponent and a page with a small scale loses no precision; u is kept apart
+//     from m because beside a large score a scale's logarithm would be rounded away.  A reference moves
+//     only when a score passes it by 2^kSlack: O and l are rescaled, and lanes compare notes, only then.
 //   K of the next tile is loaded before the softmax of this one, V of this one before its S.
 #include "fa_internal.h"
 #include "fa_paged.cuh"
@@ -45,6 +46,7 @@ constexpr int kWarps = kPagedThreads / 32;
 constexpr int kUnit = kPagedUnit;   // keys of a unit
 constexpr int kTile = 32;           // keys of a warp's tile
 constexpr float kSlack = 8.f;       // log2: weights stay below 2^8 of the reference, far inside f16
+constexpr float kNoScale = -200.f;  // stands for log2 0: below every float32's
 
 template <int D, int NT>
 struct PagedCfg {  // resident blocks per SM, as the registers allow
@@ -233,8 +235,8 @@ struct RowTile {
 template <int D, int NT>
 struct WarpState {
   float o[NT][D / 16][4];   // O^T: rows g, g + 8 of each 16-row tile, columns 2t, 2t + 1
-  float mw[NT][2];          // reference of s + log2(v_scale), all lanes of a column alike
-  float m[NT][2];           // this thread's reference of s
+  float m[NT][2];           // reference of s, all lanes of a column alike
+  float u[NT][2];           // reference of s - m + log2(v_scale), likewise
   float l[NT][2];           // this thread's sum of 2^(s - m)
 };
 
@@ -246,12 +248,11 @@ __device__ __forceinline__ void softmax_pv(WarpState<D, NT>& st, float (&s)[NT][
                                            const int (&last)[NT][2], int key0, int keys, int g, int t,
                                            volatile int* saw_nan) {
   bool raise = false;
-  float top[NT][2][2];  // per column: this thread's largest score, and with its page's scale
+  float top[NT][2][2];  // per column: this thread's largest score of each block
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float block_top[2];
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
         const float f = qs[nt][c] * ks[blk];
@@ -261,23 +262,30 @@ __device__ __forceinline__ void softmax_pv(WarpState<D, NT>& st, float (&s)[NT][
           if (EDGE && key0 + 16 * blk + 8 * r + g > last[nt][c]) x = -INFINITY;
           s[nt][blk][2 * r + c] = x;
         }
-        block_top[blk] = fmaxf(s[nt][blk][c], s[nt][blk][2 + c]);
+        top[nt][c][blk] = fmaxf(s[nt][blk][c], s[nt][blk][2 + c]);
+        // by the threshold above m, or with the scale above m + u (m = -inf: any score)
+        raise |= top[nt][c][blk] - st.m[nt][c] > kSlack + fminf(0.f, st.u[nt][c] - vs[blk]);
       }
-      top[nt][c][0] = fmaxf(block_top[0], block_top[1]);
-      top[nt][c][1] = fmaxf(block_top[0] + vs[0], block_top[1] + vs[1]);
-      raise |= top[nt][c][1] > st.mw[nt][c] + kSlack;
     }
   if (__any_sync(0xffffffffu, raise)) {  // new references, the same in all lanes of a column
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float ref = top[nt][c][1];
+        float m = fmaxf(st.m[nt][c], fmaxf(top[nt][c][0], top[nt][c][1]));
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-        ref = fmaxf(st.mw[nt][c], ref);
-        const float alpha = st.mw[nt][c] == -INFINITY ? 0.f : ex2_approx(st.mw[nt][c] - ref);
-        st.mw[nt][c] = ref;
+        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float down = st.m[nt][c] - m;  // -inf for the first score, NaN (and no other lane's sum) before it
+        const float before = st.u[nt][c] + down;
+        float u = fmaxf((top[nt][c][0] - m) + vs[0], (top[nt][c][1] - m) + vs[1]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o));
+        u = fmaxf(fmaxf(before, u), kNoScale);
+        const float alpha_l = st.m[nt][c] == -INFINITY ? 0.f : ex2_approx(down);
+        const float alpha = st.m[nt][c] == -INFINITY ? 0.f : ex2_approx(before - u);
+        st.m[nt][c] = m;
+        st.u[nt][c] = u;
+        st.l[nt][c] *= alpha_l;
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt) {
           st.o[nt][mt][c] *= alpha;
@@ -290,22 +298,16 @@ __device__ __forceinline__ void softmax_pv(WarpState<D, NT>& st, float (&s)[NT][
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float m = st.m[nt][c], l = st.l[nt][c];
-      if (top[nt][c][0] > m + kSlack) {  // also the first score of the thread (m = -inf, l = 0)
-        l = m == -INFINITY ? 0.f : l * ex2_approx(m - top[nt][c][0]);
-        m = top[nt][c][0];
-        st.m[nt][c] = m;
-      }
-      const float rm = m == -INFINITY ? 0.f : m;  // no score yet: all terms below are 0
-      const float rw = st.mw[nt][c] == -INFINITY ? 0.f : st.mw[nt][c];
+      const float m = st.m[nt][c] == -INFINITY ? 0.f : st.m[nt][c];  // no score yet: all terms below are 0
+      float l = st.l[nt][c];
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
-        const float rb = rw - vs[blk];
+        const float shift = vs[blk] - st.u[nt][c];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float x = s[nt][blk][2 * r + c];
-          l += ex2_approx(x - rm);
-          s[nt][blk][2 * r + c] = ex2_approx(x - rb);
+          const float x = s[nt][blk][2 * r + c] - m;
+          l += ex2_approx(x);
+          s[nt][blk][2 * r + c] = ex2_approx(x + shift);
         }
       }
       st.l[nt][c] = l;
@@ -446,7 +448,8 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
       for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[nt][mt][i] = 0.f;
-      st.mw[nt][0] = st.mw[nt][1] = st.m[nt][0] = st.m[nt][1] = -INFINITY;
+      st.m[nt][0] = st.m[nt][1] = -INFINITY;
+      st.u[nt][0] = st.u[nt][1] = kNoScale;
       st.l[nt][0] = st.l[nt][1] = 0.f;
     }
 
@@ -517,8 +520,8 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) next_page[blk] = page_of(key_next + kWarps * kTile + 16 * blk);
         }
-        vs[0] = __log2f(vs[0]);
-        vs[1] = __log2f(vs[1]);
+        vs[0] = fmaxf(__log2f(vs[0]), kNoScale);
+        vs[1] = fmaxf(__log2f(vs[1]), kNoScale);
         softmax_pv<D, NT, decltype(edge)::value>(st, s, qs, ks, vs, v, last, key0, keys, g, t, &sh_nan[warp]);
         key0 = key_next;
         key_next += kWarps * kTile;
@@ -528,24 +531,20 @@ __global__ void __launch_bounds__(kPagedThreads, PagedCfg<D, NT>::kPerSm) paged_
       while (key0 < key_end) one_tile(std::true_type{});
     }
 
-    // ---- join the warps: m and l over the lanes of a column, then everything in shared memory
+    // ---- join the warps: l over the lanes of a column, then everything in shared memory
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float m = st.m[nt][c];
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l = st.l[nt][c] * ex2_approx(st.m[nt][c] - ref);
+        float l = st.l[nt][c];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         if (g == 0) {
-          sh_m[warp][8 * nt + 2 * t + c] = m;
+          sh_m[warp][8 * nt + 2 * t + c] = st.m[nt][c];
           sh_l[warp][8 * nt + 2 * t + c] = l;
         }
         // O relative to m: the pages' scales come back into it here
-        const float f = st.mw[nt][c] == -INFINITY ? 0.f : exp2f(st.mw[nt][c] - ref);
+        const float f = exp2f(st.u[nt][c]);
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt) {
           st.o[nt][mt][c] *= f;

@@ -182,3 +182,40 @@ def test_nan_keys_of_every_place_in_a_tile(s, cuda_device):
             assert bool(o[expected].isnan().all()) and torch.equal(lse.cpu().isnan(), expected)
             assert torch.equal(o[~expected], ref[~expected])
     _nat().check_status(cuda_device)
+
+
+@pytest.mark.parametrize("s", SHAPES, ids=ids)
+@pytest.mark.parametrize("power", [6, 13, 20, 30, 60])
+def test_large_scores_pick_one_value(s, power, cuda_device):
+    """Scores of about 2^power: where one leads by more than 64 and more than all float32 sums can be off, o is its
+    value, rounded as a weight (2^-11), a logarithm (2^-16) and an output, whatever the scales."""
+    table, starts, pages = batch(s["lens"], s["news"], s["P"])
+    kp, vp, ks, vs = make_cache(pages, s["H_kv"], s["P"], s["D"])
+    vs = vs * (0.5 + torch.rand(vs.shape, generator=torch.Generator().manual_seed(8)))
+    q = queries(s, torch.bfloat16) * 2.0 ** power
+    o, lse = _attend(q.cuda(), _cache(*to_gpu(kp, vp, ks, vs)), table.cuda(), i32(s["lens"]), i32(starts), return_lse=True)
+    _nat().check_status(cuda_device)
+    o, lse, leading = o.double().cpu(), lse.double().cpu(), 0
+    assert bool(o.isfinite().all())
+    group, scale = s["H"] // s["H_kv"], s["D"] ** -0.5
+    for b, L in enumerate(s["lens"]):
+        own = [int(x) for x in table[b, :-(-L // s["P"])]]
+        K, V = ((x[own].double() * y[own].double()[..., None, None]).transpose(1, 2).reshape(-1, s["H_kv"], s["D"])[:L]
+                for x, y in ((kp, ks), (vp, vs)))
+        n = s["news"][b]
+        hidden = torch.arange(L)[None] >= torch.arange(L - n, L)[:, None] + 1
+        for h in range(s["H"]):
+            row = q[starts[b]:starts[b + 1], h].double()
+            x = (row @ K[:, h // group].T * scale).masked_fill(hidden, -math.inf)
+            off = (row.abs() @ K[:, h // group].abs().T * scale).masked_fill(hidden, 0).amax(1) * 2 * s["D"] * 2.0 ** -24
+            best, at = x.topk(min(2, L), 1)
+            ahead = best[:, 0] - best[:, 1] > 64 + 4 * off
+            leading += int(ahead.sum())
+            ref = V[at[:, 0], h // group]
+            bound = (2.0 ** -11 + 2.0 ** -16) * ref.abs() + 2.0 ** -60 * V.abs().max()
+            tol = half_step(q.dtype) * (ref.abs() + bound) + bound
+            got = o[starts[b]:starts[b + 1], h]
+            assert bool(((got - ref).abs() <= tol)[ahead].all()), float(((got - ref).abs() / tol)[ahead].max())
+            wide = math.log2(math.e) * (off + 2.0 ** -11) + 2.0 ** -22 * best[:, 0].abs() * math.log2(math.e)
+            assert bool(((lse[starts[b]:starts[b + 1], h] - math.log2(math.e) * best[:, 0]).abs() <= wide)[ahead].all())
+    assert leading > 10 * (power > 6)
