@@ -342,7 +342,12 @@ __global__ void __launch_bounds__(kAppendThreads, 1) append_kernel(const __grid_
     } else if (b >= p.B) {
       return;
     }
-    const int at = p.seq_lens[b] - (end - t);  // the token's place in its sequence
+    const int len = p.seq_lens[b];
+    if (len < 0) {  // not a length; far below zero the place would wrap around
+      if (threadIdx.x == 0) record_error(p.status, kDevBadIndex, b);
+      return;
+    }
+    const int at = len - (end - t);            // the token's place in its sequence
     if (at < 0) {                              // a token before the sequence's start has no place
       t += min(-at, end - t);
       if (p.offsets == nullptr) b = t;

@@ -1,0 +1,33 @@
+"""Calls of append_kv and paged_attention that the documentation allows or rules out, beside those of test_paged_gpu.py."""
+import pytest
+import torch
+
+from tests.test_paged_gpu import _append, _attend, _cache, _nat, batch, i32, make_cache, same_bytes, to_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("length", [-1, -(1 << 31) + 1, -(1 << 31)])
+def test_negative_lengths_are_reported(length, cuda_device):
+    """Also where the place of a token, its sequence's length less the tokens behind it, leaves 32 bits."""
+    nat = _nat()
+    P, H_kv, D = 16, 2, 64
+    for news in ([1, 1, 1], [2, 1, 3]):
+        table, starts, pages = batch([40, 20, 9], news, P)
+        cache = make_cache(pages, H_kv, P, D)
+        x = torch.randn(starts[-1], 4, D, device="cuda").half()
+        for offsets in (i32(starts), None):
+            if offsets is None and starts[-1] != 3:
+                continue
+            for b in range(3):
+                lens = [40, 20, 9]
+                lens[b] = length
+                got = to_gpu(*cache)
+                _append(_cache(*got), x[:, :H_kv], x[:, :H_kv], table.cuda(), i32(lens), offsets)
+                with pytest.raises(nat.KernelError, match="outside its table"):
+                    nat.check_status(cuda_device)
+                own = [int(p) for p in table[b] if p < pages]  # nothing of that sequence is written
+                assert all(same_bytes(t[own], r[own]) for t, r in zip(got, cache) if t.element_size() == 1)
+                _attend(x, _cache(*got), table.cuda(), i32(lens), offsets)
+                with pytest.raises(nat.KernelError, match="outside its table"):
+                    nat.check_status(cuda_device)
