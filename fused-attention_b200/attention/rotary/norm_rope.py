@@ -54,7 +54,7 @@ def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, e
     cos, sin:           float32 [max_pos, D/2]
     positions:          int32 / int64 [N] or [B, N], None: 0 .. N-1; with sections a leading dimension
                         of one row per axis
-    Differentiable (once) in q, k and the weights.  A position outside the tables is reported by check_status
+    Differentiable (once, in reverse mode) in q, k and the weights; dual tensors are refused.  A position outside the tables is reported by check_status
     of the binding (attention/_lib.py).
     """
     global _ops

@@ -92,6 +92,12 @@ Tensor aligned(const Tensor& x) {
   return on16(c) ? c : c.clone();
 }
 
+// Dual tensors: the kernels give no tangents, and dropping one would be silent.
+void check_no_tangent(const char* what, std::initializer_list<OptTensor> tensors) {
+  for (const OptTensor& t : tensors)
+    TORCH_CHECK(!t.has_value() || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+
 struct Turn {  // a rotation's checked arguments
   Tensor cos, sin, pos;
   int start[4] = {0, 0, 0, 0};
@@ -275,6 +281,7 @@ std::pair<Tensor, OptTensor> qk_norm_rope(const Tensor& q, const OptTensor& k_op
                                           const OptTensor& positions, const OptTensor& q_weight, const OptTensor& k_weight,
                                           double eps, bool interleaved, const Sections& sections) {
   const Tensor k = k_opt.value_or(Tensor());
+  check_no_tangent("qk_norm_rope", {q, k_opt, cos, sin, q_weight, k_weight});
   TORCH_CHECK_TYPE(half_type(q) && (!k.defined() || k.scalar_type() == q.scalar_type()), "q, k must be float16 (or both bfloat16)");
   TORCH_CHECK_VALUE(q.dim() == 4 && q.size(1) >= 1 &&
                         (!k.defined() || (k.dim() == 4 && k.size(1) >= 1 && k.size(0) == q.size(0) && k.size(2) == q.size(2) &&
@@ -348,6 +355,7 @@ void check_batch(const Tensor& kp, const Tensor& table, const Tensor& lens, cons
 void append_kv(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor& vs, const Tensor& k, const Tensor& v,
                const Tensor& table, const Tensor& lens, const OptTensor& offsets, const OptTensor& cos, const OptTensor& sin,
                const OptTensor& positions, const OptTensor& k_weight, double eps, bool interleaved, const Sections& sections) {
+  check_no_tangent("append_kv", {k, v, cos, sin, k_weight});
   TORCH_CHECK_TYPE(half_type(k) && v.scalar_type() == k.scalar_type(), "k, v must be float16 (or both bfloat16)");
   TORCH_CHECK(!at::GradMode::is_enabled() ||
                   !(k.requires_grad() || v.requires_grad() || (k_weight.has_value() && k_weight->requires_grad())),
@@ -411,6 +419,7 @@ void append_kv(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tenso
 py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor& vs,
                            const Tensor& table, const Tensor& lens, const OptTensor& offsets, std::optional<double> scale_opt,
                            const OptTensor& out_opt, bool return_lse) {
+  check_no_tangent("paged_attention", {q, kp, vp, ks, vs, out_opt});
   TORCH_CHECK_TYPE(half_type(q), "q must be float16 or bfloat16, got ", q.scalar_type());
   TORCH_CHECK(!at::GradMode::is_enabled() || !q.requires_grad(), "paged_attention has no backward: call it under torch.no_grad()");
   check_cache(kp, vp, ks, vs);
