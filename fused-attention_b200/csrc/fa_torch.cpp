@@ -92,6 +92,11 @@ Tensor aligned(const Tensor& x) {
   return on16(c) ? c : c.clone();
 }
 
+// A call writes into t: a backward pass that saved t before notices.  (Inference tensors have no version.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Dual tensors: the kernels give no tangents, and dropping one would be silent.
 void check_no_tangent(const char* what, std::initializer_list<OptTensor> tensors) {
   for (const OptTensor& t : tensors)
@@ -360,6 +365,8 @@ void append_kv(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tenso
   TORCH_CHECK(!at::GradMode::is_enabled() ||
                   !(k.requires_grad() || v.requires_grad() || (k_weight.has_value() && k_weight->requires_grad())),
               "append_kv has no backward: call it under torch.no_grad()");
+  for (const Tensor* x : {&kp, &vp, &ks, &vs})
+    TORCH_CHECK(!at::GradMode::is_enabled() || !x->requires_grad(), "append_kv writes into the cache, which must not require a gradient");
   check_cache(kp, vp, ks, vs);
   auto apart = [](const Tensor& x, const Tensor& y) {
     const uintptr_t i = reinterpret_cast<uintptr_t>(x.const_data_ptr()), j = reinterpret_cast<uintptr_t>(y.const_data_ptr());
@@ -414,6 +421,7 @@ void append_kv(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tenso
   for (int i = 0; i < 4; ++i) a.section_start[i] = t.start[i];
   a.interleaved = interleaved;
   call(fa_append_kv, a, k, "append_kv");
+  for (const Tensor* x : {&kp, &vp, &ks, &vs}) written(*x);
 }
 
 py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor& vs,
@@ -422,6 +430,8 @@ py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, 
   check_no_tangent("paged_attention", {q, kp, vp, ks, vs, out_opt});
   TORCH_CHECK_TYPE(half_type(q), "q must be float16 or bfloat16, got ", q.scalar_type());
   TORCH_CHECK(!at::GradMode::is_enabled() || !q.requires_grad(), "paged_attention has no backward: call it under torch.no_grad()");
+  TORCH_CHECK(!at::GradMode::is_enabled() || !out_opt.has_value() || !out_opt->requires_grad(),
+              "paged_attention writes into out, which must not require a gradient");
   check_cache(kp, vp, ks, vs);
   const int64_t H_kv = kp.size(1), D = kp.size(3);
   TORCH_CHECK_VALUE(q.dim() == 3 && q.size(2) == D && q.size(1) >= 1 && q.size(1) % H_kv == 0, "q must be (T, H, D=", D,
@@ -473,6 +483,7 @@ py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, 
     a.clear_unowned = !out_opt.has_value();
     a.scale = static_cast<float>(scale);
     call(fa_paged_attention, a, q, "paged_attention");
+    if (out_opt.has_value()) written(out);
   }
   if (return_lse) return py::make_tuple(out, lse);
   return py::cast(out);

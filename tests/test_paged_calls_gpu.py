@@ -31,3 +31,34 @@ def test_negative_lengths_are_reported(length, cuda_device):
                 _attend(x, _cache(*got), table.cuda(), i32(lens), offsets)
                 with pytest.raises(nat.KernelError, match="outside its table"):
                     nat.check_status(cuda_device)
+
+
+def test_writes_are_seen_by_autograd(cuda_device):
+    """The version of every tensor that a call writes moves, and of no other: a backward pass that saved `out` before
+    raises instead of reading what was written over it."""
+    P, H, H_kv, D = 16, 4, 2, 64
+    table, starts, pages = batch([40, 20], [1, 1], P)
+    tensors = to_gpu(*make_cache(pages, H_kv, P, D))
+    cache, tg, lens = _cache(*tensors), table.cuda(), i32([40, 20])
+    q, kv = torch.randn(2, H, D, device="cuda").half(), torch.randn(2, H_kv, D, device="cuda").half()
+
+    def moved(call):
+        watched = [*tensors, q, kv, tg, lens]
+        before = [t._version for t in watched]
+        call()
+        return [t._version > v for t, v in zip(watched, before)]
+
+    assert moved(lambda: _append(cache, kv, kv, tg, lens)) == [True] * 4 + [False] * 4
+    assert moved(lambda: _attend(q, cache, tg, lens)) == [False] * 8
+    assert moved(lambda: _attend(q, cache, tg, lens, out=q)) == [False] * 4 + [True] + [False] * 3
+    x = torch.randn(2, H, D, device="cuda").half().requires_grad_(True)
+    out = torch.ones(2, H, D, device="cuda").half()
+    y = x * out
+    _attend(q, cache, tg, lens, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        mine = torch.empty(2, H, D, device="cuda").half()
+    _attend(q, cache, tg, lens, out=mine)  # tensors of inference mode have no version
+    assert torch.equal(mine, out)
+    _nat().check_status(cuda_device)

@@ -39,3 +39,12 @@ def test_attention_refuses_dual_tensors(name):
         args[name] = dual(args[name])
         with pytest.raises(RuntimeError, match="forward-mode"):
             paged_attention(**args)
+
+
+def test_tensors_that_are_written_must_not_require_gradients():
+    with pytest.raises(RuntimeError, match="out, which must not require"):
+        paged_attention(**step_args(q=half(3, 4, 64), out=half(3, 4, 64).requires_grad_(True)))
+    args = step_args(k=half(3, 2, 64), v=half(3, 2, 64))
+    args["cache"].v_scales = args["cache"].v_scales.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="cache, which must not require"):
+        append_kv(**args)
