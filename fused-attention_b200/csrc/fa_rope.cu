@@ -338,11 +338,12 @@ __global__ void __launch_bounds__(kRopeThreads, 2) rope_bwd_kernel(const RopePar
           }
           const float r = rsqrtf(group_sum<LPR>(sum) * (1.f / D) + p.eps);
           const float t = group_sum<LPR>(dot) * (1.f / D) * r * r;
-          // rows outside the tensor were loaded as zeros: they add nothing to dw
+          const float ra = live && h + u < h1 ? r : 0.f;
+          // rows outside the tensor add nothing to dw (they are zeros, and r is infinite where eps is 0)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            dl[i] = fmaf(lo[i], xl[i] * r, dl[i]);
-            dh[i] = fmaf(hi[i], xh[i] * r, dh[i]);
+            dl[i] = fmaf(lo[i], xl[i] * ra, dl[i]);
+            dh[i] = fmaf(hi[i], xh[i] * ra, dh[i]);
             lo[i] = r * (lo[i] * wl[i] - xl[i] * t);
             hi[i] = r * (hi[i] * wh[i] - xh[i] * t);
           }
