@@ -58,3 +58,24 @@ def test_eps_of_zero(dtype, shape, cuda_device):
     """Odd numbers of heads and tokens: the places of a block that have no row have no part in dw."""
     case = make(*shape, dtype, torch.float32)
     both_ways(*case, 0.0, False)
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "interleaved"])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+@pytest.mark.parametrize("shape", [(2, 3, 1, 5, 64), (1, 7, 5, 33, 128), (3, 2, 2, 40, 32)], ids=str)
+def test_rows_whose_squares_leave_float32(shape, eps, interleaved, cuda_device):
+    """bf16 rows of all sizes from 2^-60 (eps 0) or 1 to 2^110, rows of ordinary size between them: as in float64, and the
+    ordinary rows' bits do not depend on their neighbours.  (append_kv squares in float64: both norms agree.)"""
+    q, k, cos, sin, pos, w, sections, dz = make(*shape, torch.bfloat16, torch.float32)
+    plain = _op()(q, k, cos, sin, pos, *w, eps=eps, interleaved=interleaved)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    powers = torch.tensor([0, 0, 0, 58, 61, 64, 90, 110] + ([-40, -50, -60] if eps == 0 else [0, 10, 20]), device="cuda")
+    parts = []
+    for x in (q, k):
+        p = powers[torch.randint(0, len(powers), x.shape[:3], device="cuda", generator=g)]
+        parts.append((p, (x.double() * torch.exp2(p.double())[..., None]).bfloat16()))
+    (pq, q2), (pk, k2) = parts
+    both_ways(q2, k2, cos, sin, pos, w, sections, dz, eps, interleaved)
+    got = _op()(q2, k2, cos, sin, pos, *w, eps=eps, interleaved=interleaved)
+    for a, b, p in ((got[0], plain[0], pq), (got[1], plain[1], pk)):
+        assert torch.equal(a[p == 0], b[p == 0])
