@@ -166,9 +166,10 @@ __device__ __forceinline__ void two_product(uint64_t a, uint64_t b, uint64_t& pr
   err = ffma2(a, b, fneg2(product));
 }
 
-// 1 / sqrt(mean square + eps) of the row whose piece x is, as a sum of two float32 (high, low).
+// 1 / sqrt(mean square + eps) of the row whose piece x is, as a sum of two float32 (high, low), for the row times `by`:
+// a power of two for rows far from 1, so that neither their products with weights nor the root's low part leave float32.
 template <int D>
-__device__ __forceinline__ float2 row_root(const uint64_t (&lo)[4], const uint64_t (&hi)[4], double eps) {
+__device__ __forceinline__ float2 row_root(const uint64_t (&lo)[4], const uint64_t (&hi)[4], double eps, float& by) {
   double sum = 0.0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -178,7 +179,11 @@ __device__ __forceinline__ float2 row_root(const uint64_t (&lo)[4], const uint64
   const double mean = group_sum<D / 16>(sum) / D + eps;
   const double guess = rsqrtf(static_cast<float>(mean));
   double r = guess * (1.5 - 0.5 * mean * guess * guess);  // one Newton step: 2^-22 -> 2^-43
-  if (!(mean > 0x1p-100 && mean < 0x1p100)) r = 1.0 / sqrt(mean);
+  by = 1.f;
+  if (!(mean > 0x1p-100 && mean < 0x1p100)) {
+    by = mean > 1.0 ? 0x1p-64f : 0x1p64f;
+    r = 1.0 / sqrt(mean) / by;
+  }
   const float high = static_cast<float>(r);
   return make_float2(high, static_cast<float>(r - high));
 }
@@ -188,9 +193,11 @@ template <int D>
 __device__ __forceinline__ void define_row(uint64_t (&lo)[4], uint64_t (&hi)[4], bool normed, bool wide_weights,
                                            const uint64_t (&wl)[4], const uint64_t (&wh)[4], bool turned,
                                            const uint64_t (&c)[4], const uint64_t (&s)[4], double eps) {
-  uint64_t root = 0, root_low = 0;
+  uint64_t root = 0, root_low = 0, by2 = 0;
   if (normed) {
-    const float2 r = row_root<D>(lo, hi, eps);
+    float by;
+    const float2 r = row_root<D>(lo, hi, eps, by);
+    by2 = f2(by, by);
     root = f2(r.x, r.x);
     root_low = f2(r.y, r.y);
   }
@@ -198,9 +205,11 @@ __device__ __forceinline__ void define_row(uint64_t (&lo)[4], uint64_t (&hi)[4],
   for (int j = 0; j < 4; ++j) {
     uint64_t a = lo[j], b = hi[j], a_low = 0, b_low = 0;
     if (normed) {  // exact with 16-bit weights
+      a = fmul2(a, by2);
+      b = fmul2(b, by2);
       if (wide_weights) {
-        two_product(lo[j], wl[j], a, a_low);
-        two_product(hi[j], wh[j], b, b_low);
+        two_product(a, wl[j], a, a_low);
+        two_product(b, wh[j], b, b_low);
       } else {
         a = fmul2(a, wl[j]);
         b = fmul2(b, wh[j]);

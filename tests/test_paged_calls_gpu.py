@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from tests.serving_util import angles, append64, tables
 from tests.test_paged_gpu import _append, _attend, _cache, _nat, batch, i32, make_cache, same_bytes, to_gpu
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,30 @@ def test_writes_are_seen_by_autograd(cuda_device):
     _attend(q, cache, tg, lens, out=mine)  # tensors of inference mode have no version
     assert torch.equal(mine, out)
     _nat().check_status(cuda_device)
+
+
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+@pytest.mark.parametrize("rotated", [False, True], ids=["normed", "normed-rotated"])
+@pytest.mark.parametrize("wtype", [torch.bfloat16, torch.float32], ids=["w16", "w32"])
+def test_appended_rows_of_all_sizes_are_normed_exactly(eps, rotated, wtype, cuda_device):
+    """bf16 key rows from 2^-120 to the type's largest number: the bytes are those of float64."""
+    P, H_kv, D = 32, 2, 64
+    lens = news = [100]
+    table, starts, pages = batch(lens, news, P)
+    g = torch.Generator().manual_seed(3)
+    powers = torch.tensor([0, 40, 62, 90, 110, 122] + ([-20, -60, -90, -120] if eps == 0 else []))
+    power = powers[torch.randint(0, len(powers), (100, H_kv, 1), generator=g)]
+    k = (torch.randn(100, H_kv, D, generator=g, dtype=torch.float64) * torch.exp2(power.double())).bfloat16()
+    k[7] = torch.finfo(torch.bfloat16).max
+    v = torch.randn(100, H_kv, D, generator=g).bfloat16()
+    w = (1 + 0.5 * torch.randn(D, generator=g)).to(wtype)
+    cos, sin = tables(100, D, "cpu")
+    c, s = angles(cos, sin, torch.arange(100), None) if rotated else (None, None)
+    cache = make_cache(pages, H_kv, P, D)
+    ref = append64(*cache, k, v, table, lens, starts, c, s, w, eps, False)
+    got = to_gpu(*cache)
+    kw = dict(cos=cos.cuda(), sin=sin.cuda()) if rotated else {}
+    _append(_cache(*got), k.cuda(), v.cuda(), table.cuda(), i32(lens), i32(starts), k_weight=w.cuda(), eps=eps, **kw)
+    _nat().check_status(cuda_device)
+    for name, a, b in zip(("k_pages", "v_pages", "k_scales", "v_scales"), got, ref):
+        assert same_bytes(a, b), (name, int((a.cpu().view(torch.uint8) != b.view(torch.uint8)).sum()))
