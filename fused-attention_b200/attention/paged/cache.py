@@ -37,8 +37,9 @@ def _load_ops():
 
 class PagedKVCache:
     """The cache's four tensors: k_pages, v_pages (torch.float8_e4m3fn [num_pages, H_kv, page_size, D], page_size 16,
-    32, 64 or 128, D 32, 64 or 128) and k_scales, v_scales (float32 [num_pages, H_kv]), all contiguous on one
-    device; appending needs keys and values that share no memory.  The operators write into these tensors."""
+    32, 64 or 128, D 32, 64 or 128; they start on 16-byte boundaries) and k_scales, v_scales (float32
+    [num_pages, H_kv]), all contiguous on one device; appending needs keys and values that share no memory.  The
+    operators write into these tensors."""
 
     __slots__ = ("k_pages", "v_pages", "k_scales", "v_scales")
 

@@ -330,10 +330,9 @@ void check_cache(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Ten
   TORCH_CHECK_VALUE((P == 16 || P == 32 || P == 64 || P == 128) && (D == 32 || D == 64 || D == 128) && kp.size(0) >= 1 &&
                         kp.size(1) >= 1 && kp.size(0) <= std::numeric_limits<int>::max(),
                     "page_size must be one of (16, 32, 64, 128) and D one of (32, 64, 128), got ", kp.sizes());
-  for (const Tensor* x : {&kp, &vp, &ks, &vs}) {
-    TORCH_CHECK_VALUE(x->device() == kp.device() && x->is_contiguous() && (reinterpret_cast<uintptr_t>(x->const_data_ptr()) & 15) == 0,
-                      "pages and scales must be contiguous on one device (", kp.device(), ") and start on 16-byte boundaries");
-  }
+  for (const Tensor* x : {&kp, &vp, &ks, &vs})
+    TORCH_CHECK_VALUE(x->device() == kp.device() && x->is_contiguous(), "pages and scales must be contiguous on one device (", kp.device(), ")");
+  TORCH_CHECK_VALUE(on16(kp) && on16(vp), "pages must start on 16-byte boundaries");
 }
 
 // The batch's tables against the cache and T tokens on `device`.

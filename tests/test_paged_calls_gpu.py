@@ -90,3 +90,27 @@ def test_appended_rows_of_all_sizes_are_normed_exactly(eps, rotated, wtype, cuda
     _nat().check_status(cuda_device)
     for name, a, b in zip(("k_pages", "v_pages", "k_scales", "v_scales"), got, ref):
         assert same_bytes(a, b), (name, int((a.cpu().view(torch.uint8) != b.view(torch.uint8)).sum()))
+
+
+def test_scales_of_a_layer_in_a_larger_tensor(cuda_device):
+    """One layer's scales of all layers', which start at any multiple of 4 bytes."""
+    P, H, H_kv, D = 16, 6, 3, 64
+    lens, news = [70, 33, 20], [3, 2, 20]
+    table, starts, pages = batch(lens, news, P, extra_pages=0 if (sum(-(-L // P) for L in lens)) % 2 else 1)
+    assert pages * H_kv % 2 == 1
+    kp, vp, ks, vs = make_cache(pages, H_kv, P, D)
+    x = torch.randn(starts[-1], H, D, device="cuda").half()
+    results = []
+    for layer in range(3):
+        scales = torch.full((2, 4, pages, H_kv), 7.0, device="cuda")
+        scales[0, layer], scales[1, layer] = ks.cuda(), vs.cuda()
+        before = scales.clone()
+        pages_of = to_gpu(kp, vp)
+        cache = _cache(*pages_of, scales[0, layer], scales[1, layer])
+        _append(cache, x[:, :H_kv], x[:, H_kv:], table.cuda(), i32(lens), i32(starts))
+        results.append((*(t.view(torch.uint8) for t in pages_of), scales[0, layer].clone(), scales[1, layer].clone(),
+                        _attend(x, cache, table.cuda(), i32(lens), i32(starts))))
+        for other in range(4):
+            assert other == layer or torch.equal(scales[:, other], before[:, other])
+    _nat().check_status(cuda_device)
+    assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))

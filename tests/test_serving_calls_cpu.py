@@ -1,0 +1,22 @@
+"""Calls around attention that are refused, or no longer refused, without a GPU: beside test_serving_cpu.py."""
+import pytest
+import torch
+
+from attention.paged.cache import PagedKVCache
+from tests.test_serving_cpu import cache_tensors
+
+
+def test_scales_may_start_anywhere():
+    """Scales are read one by one: one layer's part of all layers' scales starts at any multiple of 4 bytes."""
+    kp, vp, _, _ = cache_tensors(pages=3, H_kv=1)
+    scales = torch.zeros(2, 5, 3, 1)
+    for layer in range(5):
+        PagedKVCache(kp, vp, scales[0, layer], scales[1, layer])
+
+
+def test_pages_start_on_16_bytes():
+    kp, vp, ks, vs = cache_tensors()
+    odd = torch.zeros(kp.numel() + 8, dtype=torch.uint8)[8:].view(kp.dtype).view(kp.shape)
+    for t in ((odd, vp, ks, vs), (kp, odd, ks, vs)):
+        with pytest.raises(ValueError, match="16-byte"):
+            PagedKVCache(*t)
