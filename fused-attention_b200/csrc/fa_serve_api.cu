@@ -204,7 +204,7 @@ int fa_paged_attention(const fa_paged_args* a, int* dev_status, void* stream) {
                        a->k_scales, a->v_scales, a->block_table, a->seq_lens, a->offsets, a->dtype);
   if (rc != FA_OK) return rc;
   if (a->H < 1 || a->H % a->H_kv != 0) return FA_ERR_INVALID_ARG;
-  if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return FA_ERR_INVALID_ARG;
+  if (!(a->scale > 0.f) || !(a->scale * 1.4426950408889634f < INFINITY)) return FA_ERR_INVALID_ARG;
   if (static_cast<long long>(a->T) * a->H > (1LL << 30)) return FA_ERR_UNSUPPORTED;
   if (!aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->lse, 4) || !aligned(a->workspace, 16) ||
       !strides_ok(a->q_stride) || !strides_ok(a->out_stride))

@@ -437,8 +437,9 @@ py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, 
                     ") with H a multiple of H_kv=", H_kv, "; got ", q.sizes());
   const int64_t T = q.size(0), H = q.size(1), B = lens.dim() == 1 ? lens.size(0) : 0;
   const double scale = scale_opt.value_or(1.0 / std::sqrt(static_cast<double>(D)));
-  // as float32: what the kernel multiplies with
-  TORCH_CHECK_VALUE(static_cast<float>(scale) > 0.f && std::isfinite(static_cast<float>(scale)), "scale must be positive and finite, got ", scale);
+  // as float32, and times log2(e) in float32: what the kernel multiplies with
+  TORCH_CHECK_VALUE(static_cast<float>(scale) > 0.f && std::isfinite(static_cast<float>(scale) * 1.4426950408889634f),
+                    "scale must be positive and finite (below 2^127), got ", scale);
   TORCH_CHECK_VALUE(!out_opt.has_value() || (out_opt->sizes() == q.sizes() && out_opt->scalar_type() == q.scalar_type() && out_opt->device() == q.device()),
                     "out must be like q, ", q.sizes(), " ", q.scalar_type(), "; got ", out_opt->sizes(), " ", out_opt->scalar_type());
   check_batch(kp, table, lens, offsets, T, q.device());

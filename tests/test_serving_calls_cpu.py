@@ -3,7 +3,8 @@ import pytest
 import torch
 
 from attention.paged.cache import PagedKVCache
-from tests.test_serving_cpu import cache_tensors
+from attention.paged.paged_attention import paged_attention
+from tests.test_serving_cpu import PA, PAGED_ARGS, _packed, _rc, cache_tensors, half, step_args
 
 
 def test_scales_may_start_anywhere():
@@ -20,3 +21,10 @@ def test_pages_start_on_16_bytes():
     for t in ((odd, vp, ks, vs), (kp, odd, ks, vs)):
         with pytest.raises(ValueError, match="16-byte"):
             PagedKVCache(*t)
+
+
+def test_scales_of_scores_that_overflow_are_refused():
+    """The kernels multiply with scale log2(e): above 2^127.47 that is infinite, and every row NaN."""
+    with pytest.raises(ValueError, match="scale must be positive and finite"):
+        paged_attention(**step_args(q=half(3, 4, 64), scale=3e38))
+    assert _rc("fa_paged_attention", _packed(PAGED_ARGS, PA, scale=3e38)) == 1
