@@ -31,7 +31,8 @@ def paged_attention(q, cache, block_table, seq_lens, offsets=None, scale=None, o
 
     block_table, seq_lens, offsets: as for append_kv; seq_lens counts the new tokens
     scale:       factor of q k^T, 1 / sqrt(D) unless given
-    out:         where to write o (q itself is allowed); its rows behind offsets[B] are left as they are (without it they are 0)
+    out:         where to write o (q itself is allowed, a part of its memory is not); its rows behind offsets[B] are left as
+                 they are (without it they are 0)
     return_lse:  also return lse, float32 [T, H]: log2 of the sum of 2^(log2(e) scale q k) over the keys
     A token that sees no key gives o = 0 and lse = -inf.
     The cache's scales are finite and not negative.  A NaN in a cached value reaches the tokens that see it, no others.

@@ -7,6 +7,7 @@
 // function another 100 us a step, most of it handing the interpreter lock to the engine's thread.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -442,6 +443,9 @@ py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, 
                     "scale must be positive and finite (below 2^127), got ", scale);
   TORCH_CHECK_VALUE(!out_opt.has_value() || (out_opt->sizes() == q.sizes() && out_opt->scalar_type() == q.scalar_type() && out_opt->device() == q.device()),
                     "out must be like q, ", q.sizes(), " ", q.scalar_type(), "; got ", out_opt->sizes(), " ", out_opt->scalar_type());
+  // rows of o are written while others' q is read: o in q's place is fine, o beside it is not
+  TORCH_CHECK_VALUE(!out_opt.has_value() || at::get_overlap_status(*out_opt, q) != at::MemOverlapStatus::Partial,
+                    "out may be q itself but must not overlap it in part");
   check_batch(kp, table, lens, offsets, T, q.device());
   TORCH_CHECK_VALUE(T * H <= (1 << 30), "T * H must stay below 2^30, got ", q.sizes());
   Tensor out;

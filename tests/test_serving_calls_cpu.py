@@ -28,3 +28,13 @@ def test_scales_of_scores_that_overflow_are_refused():
     with pytest.raises(ValueError, match="scale must be positive and finite"):
         paged_attention(**step_args(q=half(3, 4, 64), scale=3e38))
     assert _rc("fa_paged_attention", _packed(PAGED_ARGS, PA, scale=3e38)) == 1
+
+
+def test_out_that_overlaps_part_of_q_is_refused():
+    """Some blocks would read queries that others have overwritten with their rows."""
+    both = half(5, 4, 64)
+    with pytest.raises(ValueError, match="overlap it in part"):
+        paged_attention(**step_args(q=both[:3], out=both[1:4]))
+    for q, out in ((both[:3], both[:3]), (half(3, 8, 64)[:, :4], half(3, 8, 64)[:, 4:])):
+        with pytest.raises(ValueError, match="CUDA device"):  # as far as a machine without one goes
+            paged_attention(**step_args(q=q, out=out))
