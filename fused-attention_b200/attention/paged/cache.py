@@ -87,7 +87,9 @@ def append_kv(cache, k, v, block_table, seq_lens, offsets=None, cos=None, sin=No
     that holds them; a page that holds older tokens keeps its scale unless the new ones need a larger
     one, and then the older ones are rounded again.  Infinities in v, and in k where it is neither normed nor
     rotated, are stored as the largest magnitude, NaN as NaN; neither changes a scale.  Tokens behind
-    offsets[B], and tokens that would lie before their sequence's start, are not written.  A page that is written must belong to one sequence of the batch.
+    offsets[B], and tokens that would lie before their sequence's start, are not written.  A page that is written
+    must belong to one sequence of the batch.  A position, page, length or offset outside its table (a negative
+    length too) is reported by check_status of the binding (attention/_lib.py).
     """
     (_ops or _load_ops()).append_kv(cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, k, v, block_table, seq_lens,
                                     offsets, cos, sin, positions, k_weight, eps, interleaved, sections)

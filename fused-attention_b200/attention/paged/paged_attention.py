@@ -35,7 +35,11 @@ def paged_attention(q, cache, block_table, seq_lens, offsets=None, scale=None, o
                  they are (without it they are 0)
     return_lse:  also return lse, float32 [T, H]: log2 of the sum of 2^(log2(e) scale q k) over the keys
     A token that sees no key gives o = 0 and lse = -inf.
-    The cache's scales are finite and not negative.  A NaN in a cached value reaches the tokens that see it, no others.
+    The cache's scales are finite and not negative, of any size.  A NaN in a cached key or value reaches the tokens that
+    see it, no others.  Scores, their sums and o's are float32; a weight is rounded to float16 (2^-11 of it), relative
+    to the token's own largest.
+    A page, length or offset outside its table is reported by check_status of the binding (attention/_lib.py), like
+    qk_norm_rope's positions.
     """
     global _ops
     if _ops is None:

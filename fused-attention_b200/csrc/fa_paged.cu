@@ -12,7 +12,7 @@
 //     of the call, in order, are cut into equal contiguous shares, one per block of a single wave: no block has more than its share however
 //     ragged the lengths are, and there is no atomic and no order that depends on timing.  A tile
 //     that is cut is written as partial results and joined by the second kernel, in a fixed order.
-//     Measured with D = 128: 128 sequences of 4096 keys and 8 K/V heads 176 us, 6.1 TB/s or 93 % of the
+//     Measured with D = 128: 128 sequences of 4096 keys and 8 K/V heads 174 us, 6.2 TB/s or 94 % of the
 //     measured copy rate; 32 of up to 8192 65 us, 81 %; a fixed cost of about 9 us (two launches,
 //     five dependent reads to the first key, the join) is what short histories pay.
 //   * Warps.  The four warps of a block take 32-key tiles of a share in turn, each with its own
@@ -22,9 +22,8 @@
 //     wastes nothing.  The k index of S^T (the head dim) and the m index of O^T (again the head
 //     dim) may be permuted freely, which lets a thread take 16-byte pieces of a cached row and turn
 //     bytes into operands with one conversion per pair.  S^T leaves the instruction as an 8 x 8 tile
-//     whose transpose is the second product's operand (movmatrix).  The e4m3 form of mma.sync would
-//     spare the conversions, but it is not a machine instruction here (it expands into conversions and
-//     f16 products; measured 74 us instead of 68 for 32 sequences of up to 8192).
+//     whose transpose is the second product's operand (movmatrix).  The e4m3 form of mma.sync needs no
+//     conversions but was slower (74 us instead of 68 for 32 sequences of up to 8192).
 //   * Types.  e4m3 is exact in f16, so K and V lose nothing; bf16 queries are brought into f16's
 //     range by a power of two per row (exact).  A row has two references, float32: m of its scores, which
 //     its sum l is relative to, and u of s - m + log2(v_scale).  P is f16, 2^(s - m + log2(v_scale) - u), so
@@ -80,7 +79,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// Read-once cache data: no reuse in L1, first to leave L2.
+// Read-once cache data: not kept in L1.
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   if constexpr (N == 4) {

@@ -15,7 +15,7 @@
 // pairs a lane needs are all its own, so only the row sums cross lanes (log2(D/16) shuffles).
 // kUnroll rows are loaded before the first is used.  Few tokens are spread out by giving each group
 // fewer heads (the host picks heads per group).  Measured, bf16, D = 128, 32 + 8 heads: forward over 32768
-// tokens 117 us, 5.9 TB/s or 90 % of the measured copy rate; over 8192 tokens forward 34 us, backward 58 us.
+// tokens 117 us, 5.9 TB/s or 90 % of the measured copy rate; over 8192 tokens forward 34 us, backward 56 us.
 // The weight gradients are summed in registers over a block's rows, then over the block's groups,
 // and written as one row per block; a second kernel adds those rows in a fixed order, so results do
 // not depend on timing.
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kRopeThreads, 2) rope_bwd_kernel(const RopePar
         }
       }
       if constexpr (BF16) {
-        // Not inside the rows' own code: a branch there keeps the two rows from overlapping (8192 tokens: 72 us, now 58).
+        // Not inside the rows' own code: a branch there keeps the two rows from overlapping (8192 tokens: 72 us, now 56).
         if (__any_sync(0xffffffffu, again)) {
 #pragma unroll 1
           for (int k = h; k < min(h1, h + kUnroll); ++k) {
