@@ -51,8 +51,8 @@ constexpr int kRegsOther = 64;
 static_assert(256 * kRegsOther + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split");
 constexpr int kSoftmaxCopy = 1;  // the softmax warpgroups' own copy of the bounded-wait loop
 // Of 16 exp2 pairs on interior tiles, those on the FMA pipe.  The conversions share that pipe's issue slots, so fewer
-// pay than in the dense forward: chunks of 1024, 437 and 1024 tokens behind up to 8192 keys take 310 us with one, 312 with
-// two; with pages of 16 keys 587 and 601 us for 4736 tokens behind 8192.
+// pay than in the dense forward: chunks of 1024, 437 and 1024 tokens behind up to 8192 keys take 303 us with one, 307 with
+// two; with pages of 16 keys 573 and 592 us for 4736 tokens behind 8192.
 constexpr int kPolyPairs = 1;
 // log2 of a value's scale is taken to be at least this far below the row's best weight: then p' of a score next to m is
 // 2^-60, which f16 rounds to 0 as it would the smaller exact one, while float32 still holds what l needs of it.
@@ -243,10 +243,11 @@ __device__ __forceinline__ ChunkWork find_work(const PagedParams& p, int* words)
 
 // One tile of a row's softmax with scores of any size, which are rounded before the reference is subtracted: the
 // same sums as in the kernel's loop, through TMEM in pieces of 32 columns.  factors: the segments' key scales, then
-// log2 of their value scales; keys from `hidden` on are not seen.
+// log2 of their value scales; keys from `hidden` on are not seen.  The row's m, u and l go in and come back by value: by
+// reference the kernel's loop keeps them in memory (chunks of 1024 behind 8192 keys 312 us instead of 303).
 template <int D, int kSeg>
-__device__ __noinline__ void large_tile(uint32_t t_s, uint32_t t_o, const float* factors, float row_factor, int hidden,
-                                        bool first, float& m, float& u, float& l) {
+__device__ __noinline__ float3 large_tile(uint32_t t_s, uint32_t t_o, const float* factors, float row_factor, int hidden,
+                                          bool first, float m, float u, float l) {
   constexpr int kSegs = kBN / kSeg, kPiece = kSeg < 32 ? kSeg : 32;
   uint32_t x[32];
   float top = -INFINITY;
@@ -293,9 +294,7 @@ __device__ __noinline__ void large_tile(uint32_t t_s, uint32_t t_o, const float*
     }
     tmem_st16(t_s + c * 16, pk);  // over columns that have been read
   }
-  l = l * (up ? ex2_approx(m - m_new) : 1.f) + sum;
-  m = m_new;
-  u = u_new;
+  return make_float3(m_new, u_new, l * (up ? ex2_approx(m - m_new) : 1.f) + sum);
 }
 
 // kSeg: keys that share their factors for sure, the page size up to 64.
@@ -629,7 +628,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const PagedPar
         tc_fence_after();
         const int kbase = j * kBN;
         if (large) {
-          large_tile<D, kSeg>(tS, tO, tile_factors, row_factor, last + 1 - kbase, j == 0, m, u, l);
+          const float3 state = large_tile<D, kSeg>(tS, tO, tile_factors, row_factor, last + 1 - kbase, j == 0, m, u, l);
+          m = state.x;
+          u = state.y;
+          l = state.z;
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(BAR(BAR_PFULLA + t));
@@ -809,11 +811,11 @@ static long long chunk_blocks(const PagedParams& p) {
 }
 
 // Which kernel takes a call, by the two's times for its 128-key tiles.  The split kernel spends c1 = 7 ns of the whole GPU
-// on 16 rows and 128 keys at D = 128 (4.2 ns at D = 64), the chunk kernel c2 of one SM on a block's rows: 2.2 us
-// with up to 128 of them, 2.6 to 2.8 with more.  The border is c2 / c1 = 320 at D = 128 and 400 below.  Measured at
-// D = 128, 8 K/V heads, groups of 4, 8192 keys, chunk / split in us: 16 x 16 tokens 151 / 235, 16 x 10 tokens 148 / 183,
-// 1 x 256 tokens 170 / 200, 1 x 208 tokens 171 / 169, 1 x 160 tokens (the border) 170 / 135, 4 x 16 tokens 144 / 71, 1 x 64
-// tokens 170 / 67: with one sequence the border is low, with many it is not.  Only averages are known here:
+// on 16 rows and 128 keys at D = 128 (4.2 ns at D = 64), the chunk kernel c2 of one SM on a block's rows: 2.1 us
+// with up to 128 of them, 2.5 to 2.8 with more.  The border is c2 / c1 = 320 at D = 128 and 400 below.  Measured at
+// D = 128, 8 K/V heads, groups of 4, 8192 keys, chunk / split in us: 16 x 16 tokens 147 / 226, 16 x 10 tokens 144 / 176,
+// 1 x 256 tokens 167 / 194, 1 x 208 tokens 166 / 163, 1 x 160 tokens (the border) 167 / 131, 4 x 16 tokens 140 / 69, 1 x 64
+// tokens 166 / 64: with one sequence the border is low, with many it is not.  Only averages are known here:
 // sequences' lengths are on the device.
 bool use_chunk(const PagedParams& p, int D) {
   if (chunk_blocks(p) > 0x7fffffffLL) return false;
